@@ -55,6 +55,11 @@ enum {
     WK_COMPLEX = 10, /* WK_COMPLEX + real id */
     WK_DTYPE_COUNT = 20
 };
+/* Element formats beyond the reference's twenty: IEEE half, bfloat16 and the 8-bit format with four exponent and
+ * three fraction bits (largest value 448, one NaN, no infinities).  wk_dtype_size, wk_transpose, the copies and the
+ * entry points under "the token end of a network" take them; every other entry point answers
+ * WK_E_TYPE_NOT_SUPPORTED. */
+enum { WK_F16 = 32, WK_BF16 = 33, WK_F8E4M3 = 34 };
 
 /* src/blas/gemm.zig:25-29 `Operation` */
 enum { WK_OP_NO_TRANSPOSE = 0, WK_OP_TRANSPOSE = 1 };
@@ -288,6 +293,76 @@ int  wk_to_complex(wk_stream *s, int real_dtype, const uint64_t shape3[3], const
                    uint64_t src_slice_pitch, void *dst, uint64_t dst_row_pitch, uint64_t dst_slice_pitch, int space);
 int  wk_to_real(wk_stream *s, int real_dtype, const uint64_t shape3[3], const void *src, uint64_t src_row_pitch,
                 uint64_t src_slice_pitch, void *dst, uint64_t dst_row_pitch, uint64_t dst_slice_pitch, int space);
+
+/* ---- the token end of a network ------------------------------------------------------------------
+ * No counterpart in the reference, whose only loss is mse.  Dropout, products of 8-bit floating point with a
+ * scale for every block of 128 elements of k, and log probabilities of given tokens with their gradient. */
+
+/* Dropout: y = x / (1 - p) where an element is kept, 0 where it is dropped (whatever x holds there).  Element i of
+ * the logical {depth, rows, cols} region, counted row by row whatever the pitches, is kept when its 32-bit
+ * word is at least floor(p 2^32); the words are those of the counter-based generator Philox4x32 with seven rounds
+ * (Salmon et al., "Parallel random numbers: as easy as 1, 2, 3", 2011): words 4b .. 4b + 3 come from the counter
+ * {b low, b high, n low, n high} under the key {seed low, seed high}, with n = offset + *dev_step.  The mask is
+ * never stored: the backward pass is the same call on the gradient, with the same p, seed and n.
+ * dev_step (NULL: 0) is one u64 in device memory, read when the kernel runs: a program that replays a captured
+ * call counts there to get a new mask with each replay.
+ * f32, f64, f16, bf16; the product is taken in 32 bits (f64: 64) and rounded once.  0 <= p <= 1.
+ * y may be x with the same pitches; otherwise the two must not overlap. */
+int  wk_dropout(wk_stream *s, int dtype, const uint64_t shape3[3], const void *x, uint64_t x_row_pitch, uint64_t x_slice_pitch,
+                void *y, uint64_t y_row_pitch, uint64_t y_slice_pitch, double p, uint64_t seed, uint64_t offset,
+                const uint64_t *dev_step);
+
+/* Quantiser of the products below: 8-bit codes (WK_F8E4M3) and one f32 scale for each block of block_rows x 128 elements
+ * of x [rows x cols]; x is about code * scale.  block_rows 1 (activations) or 128 (weights).  scales is
+ * [ceil(rows / block_rows) x ceil(cols / 128)] with scale_pitch elements between its rows.  The scale is
+ * the least power of two (2^-126 or more) under which the block's largest magnitude fits into 448, so the division is
+ * exact and each code is x / scale rounded once, to nearest, ties to even; a block of zeros has scale 1.  A block that
+ * holds a NaN or an infinity gets a NaN scale and NaN codes.  x: f32, f16, bf16. */
+int  wk_f8_quantize(wk_stream *s, int dtype, uint64_t rows, uint64_t cols, const void *x, uint64_t pitch, uint64_t block_rows,
+                    void *q, uint64_t q_pitch, float *scales, uint64_t scale_pitch);
+
+/* C = act(A B^T + bias) of 8-bit operands (WK_F8E4M3), what Linear.forward computes:
+ *   C[m][n] = act( sum over blocks b of k: a_scales[m][b] * b_scales[n / 128][b] * sum_{k in b} A[m][k] B[n][k]  + bias[n] )
+ * A is M x K, B is N x K (a weight matrix as Linear keeps it), both row-major; blocks are 128 elements of k, the last
+ * one shorter when K is no multiple.  Any f32 scales are taken, not only the quantiser's.  Sums are held in
+ * 32 bits; C is f32, f16 or bf16 (out_dtype), rounded once.  For f32 every product enters its sum whole; for the 16-bit types
+ * the 8-bit matrix instructions are used, which cut each product at 2^-13 of the largest of the eight consecutive ones that
+ * it is summed with (1.5e-5 of a result on normally distributed operands, where a half step of bf16 is 4e-3 and of f16
+ * 5e-4).  bias: N f32 or NULL; kind: WK_ACT_*.
+ * Rows of A and B on 16-byte boundaries (bases and leading dimensions multiples of 16) are read 16 bytes at a time, any
+ * others byte by byte.  B turned around (for the gradient of the input) is wk_transpose of its codes and, for
+ * 128 x 128 blocks, of its scales. */
+int  wk_gemm_f8(wk_stream *s, uint64_t M, uint64_t N, uint64_t K, const void *A, uint64_t lda, const float *a_scales,
+                uint64_t a_scale_pitch, const void *B, uint64_t ldb, const float *b_scales, uint64_t b_scale_pitch, int out_dtype,
+                void *C, uint64_t ldc, const float *bias, int kind);
+
+/* Log probabilities of given tokens: for each row x of logits [rows x vocab], with one pass over it,
+ *   lse = ln sum_j exp(x_j)   logprob = x_target - lse   entropy = lse - sum_j p_j x_j,  p_j = exp(x_j - lse)
+ * and the `top` likeliest tokens (0 <= top <= WK_TOKEN_TOP_MAX, top <= vocab), likeliest first, equal logits by lowest
+ * index, as ids (i32) and log probabilities, `top` to a row.  logits: f32, f64, f16, bf16; everything is computed and returned in f32 (f64
+ * for f64).  targets are i32 or i64 (target_dtype).  Any of logprob, lse, entropy may be NULL (targets too,
+ * without logprob), but not all with top 0.
+ *   - a negative target means none: logprob 0.  One that is not below vocab gives NaN (nothing is read there).
+ *   - logits of -inf are masked: they count nothing and are no alternatives; where fewer than `top` others
+ *     remain, the rest of the row's ids is -1 with log probability -inf.
+ *   - a row that its mask leaves empty has lse -inf, logprob -inf, entropy 0; a row that holds NaN or +inf has NaN in
+ *     lse, logprob, entropy and top_logprobs, and ids -1.
+ * vocab < 2^31.  workspace (16-byte aligned device memory of at least wk_token_logprobs_workspace_bytes(), or NULL) lets few long
+ * rows be cut over more work-groups; it is overwritten by every call that uses it, so calls sharing one must be ordered. */
+#define WK_TOKEN_TOP_MAX 64
+size_t wk_token_logprobs_workspace_bytes(int dtype, uint64_t rows, uint64_t vocab, uint32_t top);
+int  wk_token_logprobs(wk_stream *s, int dtype, uint64_t rows, uint64_t vocab, const void *logits, uint64_t pitch, const void *targets,
+                       int target_dtype, void *logprob, void *lse, void *entropy, uint32_t top, int32_t *top_ids, void *top_logprobs,
+                       void *workspace, size_t workspace_bytes);
+/* Its backward pass, from the lse (and entropy) that the forward pass returned:
+ *   logits_grad_j = logprob_grad * ((j == target) - p_j) - entropy_grad * p_j * (x_j - lse + entropy)
+ * with one value of logprob_grad and entropy_grad to a row (f32, f64 for f64 logits); either may be NULL (targets too without
+ * the first, entropy without the second), not both.  logits_grad is of the logits' type and may be logits itself
+ * (same pitch).  A row without a target has no first term; masked logits get 0 (the target itself: logprob_grad); a row with
+ * lse -inf gets zeros, one with a target that is not below vocab, or whose lse is NaN, gets NaN. */
+int  wk_token_logprobs_grad(wk_stream *s, int dtype, uint64_t rows, uint64_t vocab, const void *logits, uint64_t pitch,
+                            const void *targets, int target_dtype, const void *lse, const void *entropy, const void *logprob_grad,
+                            const void *entropy_grad, void *logits_grad, uint64_t grad_pitch);
 
 #ifdef __cplusplus
 }

@@ -101,6 +101,12 @@ SIGNATURES = {
     "wk_random_hash": (u64, [u64, u64]),
     "wk_to_complex": (ci, [vp, ci, u64p, vp, u64, u64, vp, u64, u64, ci]),
     "wk_to_real": (ci, [vp, ci, u64p, vp, u64, u64, vp, u64, u64, ci]),
+    "wk_dropout": (ci, [vp, ci, u64p, vp, u64, u64, vp, u64, u64, ctypes.c_double, u64, u64, vp]),
+    "wk_f8_quantize": (ci, [vp, ci, u64, u64, vp, u64, u64, vp, u64, vp, u64]),
+    "wk_gemm_f8": (ci, [vp, u64, u64, u64, vp, u64, vp, u64, vp, u64, vp, u64, ci, vp, u64, vp, ci]),
+    "wk_token_logprobs_workspace_bytes": (sz, [ci, u64, u64, ctypes.c_uint32]),
+    "wk_token_logprobs": (ci, [vp, ci, u64, u64, vp, u64, vp, ci, vp, vp, vp, ctypes.c_uint32, vp, vp, vp, sz]),
+    "wk_token_logprobs_grad": (ci, [vp, ci, u64, u64, vp, u64, vp, ci, vp, vp, vp, vp, vp, u64]),
 }
 
 _lib = None

@@ -63,7 +63,7 @@ int build_problem(GemmProblem &p, int dtype, int op_a, int op_b, uint64_t M, uin
                   const void *host_alpha, const void *A, uint64_t lda, const void *B, uint64_t ldb,
                   const void *host_beta, void *C, uint64_t ldc) {
     const size_t es = wk_dtype_size(dtype);
-    if (es == 0) return WK_E_TYPE_NOT_SUPPORTED;
+    if (es == 0 || dtype >= WK_DTYPE_COUNT) return WK_E_TYPE_NOT_SUPPORTED;
     if ((op_a != WK_OP_NO_TRANSPOSE && op_a != WK_OP_TRANSPOSE) || (op_b != WK_OP_NO_TRANSPOSE && op_b != WK_OP_TRANSPOSE))
         return WK_E_INVALID_VALUE;
     if (!M || !N || !K || !A || !B || !C) return WK_E_INVALID_VALUE;

@@ -53,6 +53,8 @@ int wk_abi_version(void) { return WK_ABI_VERSION; }
 
 size_t wk_dtype_size(int dtype) {
     static const size_t real_size[10] = {1, 1, 2, 2, 4, 4, 8, 8, 4, 8};
+    if (dtype == WK_F16 || dtype == WK_BF16) return 2;
+    if (dtype == WK_F8E4M3) return 1;
     if (dtype < 0 || dtype >= WK_DTYPE_COUNT) return 0;
     return dtype >= WK_COMPLEX ? 2 * real_size[dtype - WK_COMPLEX] : real_size[dtype];
 }

@@ -14,15 +14,20 @@ from ._capi import check
 
 REAL_NAMES = ["i8", "u8", "i16", "u16", "i32", "u32", "i64", "u64", "f32", "f64"]
 DTYPE_NAMES = REAL_NAMES + ["c" + n for n in REAL_NAMES]
+# element formats beyond the reference's twenty; numpy holds bf16 and f8e4m3 as their bits
+EXTRA_DTYPES = {"f16": 32, "bf16": 33, "f8e4m3": 34}
+_NP_EXTRA = {"f16": np.float16, "bf16": np.uint16, "f8e4m3": np.uint8}
 _NP_REAL = [np.int8, np.uint8, np.int16, np.uint16, np.int32, np.uint32, np.int64, np.uint64,
             np.float32, np.float64]
 
 
 def dtype_id(name: str) -> int:
-    return DTYPE_NAMES.index(name)
+    return EXTRA_DTYPES[name] if name in EXTRA_DTYPES else DTYPE_NAMES.index(name)
 
 
 def real_np_dtype(name: str) -> np.dtype:
+    if name in _NP_EXTRA:
+        return np.dtype(_NP_EXTRA[name])
     return np.dtype(_NP_REAL[dtype_id(name) % 10])
 
 
@@ -52,6 +57,13 @@ def scalar_bytes(name: str, value):
     else:
         arr = np.array(vals, dtype=rd)
     return ctypes.create_string_buffer(arr.tobytes(), arr.nbytes)
+
+
+def _address(buf):
+    """The device address of a DeviceBuffer, of anything with data_ptr(), or a plain address; None stays None."""
+    if buf is None or isinstance(buf, int):
+        return buf
+    return buf.data_ptr() if hasattr(buf, "data_ptr") else buf.ptr
 
 
 class Device:
@@ -130,6 +142,45 @@ class Device:
         s3 = (ctypes.c_uint64 * 3)(*shape3)
         check(self.lib.wk_axpy(self.stream, dtype_id(dtype), s3, x.ptr, xrp, xsp, y.ptr, yrp, ysp,
                                ctypes.cast(a, ctypes.c_void_p) if a is not None else None), "wk_axpy")
+
+    # -- the token end of a network ---------------------------------------------------------
+    # Buffers: DeviceBuffers, device addresses, or objects with data_ptr() whose memory is on this device and ready on
+    # this stream (work of another stream on them is the caller's to wait for).
+    def dropout(self, dtype: str, shape3, x, xrp: int, xsp: int, y, yrp: int, ysp: int, p: float, seed: int, offset: int = 0,
+                step=None) -> None:
+        """wk_dropout; the backward pass is the same call on the gradient."""
+        check(self.lib.wk_dropout(self.stream, dtype_id(dtype), (ctypes.c_uint64 * 3)(*shape3), _address(x), xrp, xsp, _address(y), yrp, ysp,
+                                  p, seed, offset, _address(step)), "wk_dropout")
+
+    def f8_quantize(self, dtype: str, rows: int, cols: int, x, pitch: int, block_rows: int, q, q_pitch: int, scales,
+                    scale_pitch: int) -> None:
+        """wk_f8_quantize: 8-bit codes and a scale for each block of block_rows (1 or 128) x 128 elements."""
+        check(self.lib.wk_f8_quantize(self.stream, dtype_id(dtype), rows, cols, _address(x), pitch, block_rows, _address(q), q_pitch,
+                                      _address(scales), scale_pitch), "wk_f8_quantize")
+
+    def gemm_f8(self, M: int, N: int, K: int, A, lda: int, a_scales, a_scale_pitch: int, B, ldb: int, b_scales, b_scale_pitch: int,
+                out_dtype: str, C, ldc: int, bias=None, kind: int = -1) -> None:
+        """wk_gemm_f8: C = act(A B^T + bias) of 8-bit operands with block scales."""
+        check(self.lib.wk_gemm_f8(self.stream, M, N, K, _address(A), lda, _address(a_scales), a_scale_pitch, _address(B), ldb,
+                                  _address(b_scales), b_scale_pitch, dtype_id(out_dtype), _address(C), ldc, _address(bias), kind), "wk_gemm_f8")
+
+    def token_logprobs_workspace_bytes(self, dtype: str, rows: int, vocab: int, top: int = 0) -> int:
+        return int(self.lib.wk_token_logprobs_workspace_bytes(dtype_id(dtype), rows, vocab, top))
+
+    def token_logprobs(self, dtype: str, rows: int, vocab: int, logits, pitch: int, targets, target_dtype: str = "i32", logprob=None,
+                       lse=None, entropy=None, top: int = 0, top_ids=None, top_logprobs=None, workspace=None,
+                       workspace_bytes: int = 0) -> None:
+        """wk_token_logprobs; outputs that are None are not computed."""
+        check(self.lib.wk_token_logprobs(self.stream, dtype_id(dtype), rows, vocab, _address(logits), pitch, _address(targets),
+                                         dtype_id(target_dtype), _address(logprob), _address(lse), _address(entropy), top,
+                                         _address(top_ids), _address(top_logprobs), _address(workspace), workspace_bytes), "wk_token_logprobs")
+
+    def token_logprobs_grad(self, dtype: str, rows: int, vocab: int, logits, pitch: int, targets, target_dtype: str, lse, entropy,
+                            logprob_grad, entropy_grad, logits_grad, grad_pitch: int) -> None:
+        """wk_token_logprobs_grad: the gradient of the logits from those of the log probabilities and entropies."""
+        check(self.lib.wk_token_logprobs_grad(self.stream, dtype_id(dtype), rows, vocab, _address(logits), pitch, _address(targets),
+                                              dtype_id(target_dtype), _address(lse), _address(entropy), _address(logprob_grad),
+                                              _address(entropy_grad), _address(logits_grad), grad_pitch), "wk_token_logprobs_grad")
 
 
 class DeviceBuffer:

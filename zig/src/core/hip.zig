@@ -119,3 +119,19 @@ pub extern fn wk_to_complex(s: *Stream, real_dtype: c_int, shape3: *const [3]u64
 pub extern fn wk_to_real(s: *Stream, real_dtype: c_int, shape3: *const [3]u64, src: *const anyopaque, src_row_pitch: u64,
     src_slice_pitch: u64, dst: *anyopaque, dst_row_pitch: u64, dst_slice_pitch: u64, space: c_int) c_int;
 pub extern fn wk_random_hash(index: u64, seed: u64) u64;   // host copy of the device hash, for tests
+
+// ---- the token end of a network: dropout, 8-bit products with block scales, token log probabilities ----
+pub extern fn wk_dropout(s: *Stream, dtype: c_int, shape3: *const [3]u64, x: *const anyopaque, x_row_pitch: u64, x_slice_pitch: u64,
+    y: *anyopaque, y_row_pitch: u64, y_slice_pitch: u64, p: f64, seed: u64, offset: u64, dev_step: ?*const u64) c_int;
+pub extern fn wk_f8_quantize(s: *Stream, dtype: c_int, rows: u64, cols: u64, x: *const anyopaque, pitch: u64, block_rows: u64,
+    q: *anyopaque, q_pitch: u64, scales: [*]f32, scale_pitch: u64) c_int;
+pub extern fn wk_gemm_f8(s: *Stream, m: u64, n: u64, k: u64, a: *const anyopaque, lda: u64, a_scales: [*]const f32, a_scale_pitch: u64,
+    b: *const anyopaque, ldb: u64, b_scales: [*]const f32, b_scale_pitch: u64, out_dtype: c_int, c: *anyopaque, ldc: u64,
+    bias: ?[*]const f32, kind: c_int) c_int;
+pub extern fn wk_token_logprobs_workspace_bytes(dtype: c_int, rows: u64, vocab: u64, top: u32) usize;
+pub extern fn wk_token_logprobs(s: *Stream, dtype: c_int, rows: u64, vocab: u64, logits: *const anyopaque, pitch: u64,
+    targets: ?*const anyopaque, target_dtype: c_int, logprob: ?*anyopaque, lse: ?*anyopaque, entropy: ?*anyopaque, top: u32,
+    top_ids: ?[*]i32, top_logprobs: ?*anyopaque, workspace: ?*anyopaque, workspace_bytes: usize) c_int;
+pub extern fn wk_token_logprobs_grad(s: *Stream, dtype: c_int, rows: u64, vocab: u64, logits: *const anyopaque, pitch: u64,
+    targets: ?*const anyopaque, target_dtype: c_int, lse: *const anyopaque, entropy: ?*const anyopaque, logprob_grad: ?*const anyopaque,
+    entropy_grad: ?*const anyopaque, logits_grad: *anyopaque, grad_pitch: u64) c_int;
