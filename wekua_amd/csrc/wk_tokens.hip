@@ -20,6 +20,7 @@ template <> struct stat_of<double> { using type = double; };
 
 constexpr uint32_t TOP_MAX = WK_TOKEN_TOP_MAX;
 static_assert(TOP_MAX == 64, "one alternative per lane");
+constexpr uint32_t MAX_PARTS = 64; // of a row: one per lane when they are joined
 
 __device__ __forceinline__ float lowest(float) { return -__builtin_inff(); }
 __device__ __forceinline__ double lowest(double) { return -__builtin_inf(); }
@@ -54,24 +55,62 @@ template <typename A> __device__ __forceinline__ Stats<A> join(Stats<A> a, Stats
     return {m, a.s + b.s, a.u + b.u};
 }
 
-// A wavefront's best values, lane l the l-th best with its index; lanes without one hold -inf.
+__device__ __forceinline__ int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ float lane_of(float v, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane)); }
+__device__ __forceinline__ double lane_of(double v, int lane) {
+    return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), lane), __builtin_amdgcn_readlane(__double2loint(v), lane));
+}
+// each lane's lower neighbour's value (lane 0: its own)
+__device__ __forceinline__ int from_below(int v) { return __builtin_amdgcn_update_dpp(v, v, 0x138 /* wave_shr:1 */, 0xf, 0xf, false); }
+__device__ __forceinline__ float from_below(float v) { return __int_as_float(from_below(__float_as_int(v))); }
+__device__ __forceinline__ double from_below(double v) { return __hiloint2double(from_below(__double2hiint(v)), from_below(__double2loint(v))); }
+// the next value below a finite one; -inf stays
+__device__ __forceinline__ double just_below(double v) {
+    const long long b = __double_as_longlong(v);
+    return v == lowest(v) ? v : v == 0.0 ? __longlong_as_double((long long)0x8000000000000001ull) : __longlong_as_double(b > 0 ? b - 1 : b + 1);
+}
+
+// A wavefront's best values, lane l the l-th best with its index; lanes without one hold -inf and -1.
 template <typename A> struct Best {
     A v;
     int32_t id;
 };
 
-// Puts (v, id), the same in every lane, into the list; equal values that are in it already stay in front.
+// Puts (v, id), the same in every lane and v > -inf, into the list, behind equal values that are in it already.
 template <typename A> __device__ __forceinline__ void insert(Best<A> &b, A v, int32_t id, uint32_t lane) {
-    const uint32_t pos = (uint32_t)__popcll(__ballot(b.v >= v && b.id >= 0));
-    const A up = __shfl_up(b.v, 1);
-    const int32_t up_id = __shfl_up(b.id, 1);
-    if (lane == pos) {
-        b.v = v;
-        b.id = id;
-    } else if (lane > pos) {
-        b.v = up;
-        b.id = up_id;
+    const uint32_t pos = (uint32_t)__popcll(__ballot(b.v >= v));
+    const A up = from_below(b.v);
+    const int32_t up_id = from_below(b.id);
+    b.v = lane > pos ? up : lane == pos ? v : b.v;
+    b.id = lane > pos ? up_id : lane == pos ? id : b.id;
+}
+
+// A value that at least `top` of the wavefront's values are above, as high as it can be had cheaply: just below the top-th
+// largest of the lanes' maxima (-inf where so many lanes have none).  In f32 a lane's place is found by whole-number
+// comparisons of the value's order with the lane in its low six bits, which lowers the bar by up to 2^-16 of it.
+__device__ __forceinline__ float first_bar(float cm, uint32_t top, uint32_t lane) {
+    const uint32_t bits = __float_as_uint(cm);
+    const uint32_t order = (bits >> 31 ? ~bits : bits | 0x80000000u), key = (order & ~63u) | (63u - lane);
+    uint32_t above = 0;
+#pragma unroll 16
+    for (int l = 0; l < 64; ++l) above += (uint32_t)__builtin_amdgcn_readlane((int)key, l) > key;
+    const uint32_t k = (uint32_t)__builtin_amdgcn_readlane((int)(order & ~63u), __builtin_ctzll(__ballot(above == top - 1)));
+    const uint32_t low = k - 64; // a value before it (one step before +0 would be -0, its equal)
+    const float v = __uint_as_float(low >> 31 ? low & 0x7fffffffu : ~low);
+    return v == v ? v : lowest(v);
+}
+__device__ __forceinline__ double first_bar(double cm, uint32_t top, uint32_t lane) {
+    uint32_t above = 0;
+    for (int l = 0; l < 64; ++l) {
+        const double other = lane_of(cm, l);
+        above += other > cm || (other == cm && (uint32_t)l < lane);
     }
+    return just_below(lane_of(cm, __builtin_ctzll(__ballot(above == top - 1))));
+}
+
+// whether (v, id) comes before (w, id_w) among the alternatives; id < 0: no value there, behind all others
+template <typename A> __device__ __forceinline__ bool before(A v, int32_t id, A w, int32_t id_w) {
+    return id >= 0 && (id_w < 0 || v > w || (v == w && id < id_w));
 }
 
 template <typename T, int N> __device__ __forceinline__ void load_n(const T *p, uint32_t left, T raw[N]) {
@@ -119,8 +158,12 @@ template <typename A> __device__ __forceinline__ void finish_top(const Outputs<A
     o.top_logprobs[row * top + place] = bad ? A(__builtin_nanf("")) : none ? lowest(A(0)) : (v - st.m) - log(st.s);
 }
 
-// One row (or part of a row) over `threads` = 64 * WAVES threads of a work-group.  A part leaves its statistics and its
-// candidates in `ws`; a whole row is finished here.
+// One row, or a part of one, over the 64 * WAVES threads of a work-group (WAVES = 1: four rows to a work-group).  A part
+// leaves its statistics and its alternatives in `ws`; a whole row is finished here.
+//
+// A lane takes DEEP x 16 bytes a step, all loads issued before any is used.  An alternative enters the list in ~100 cycles of the
+// whole wavefront, so few should: in the first step the top-th largest of the lanes' maxima is already a bar
+// under which nothing can be among the best (at least `top` values reach it), afterwards the list's last value is.
 template <typename T, int WAVES, bool TOP>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void logprobs_kernel(const T *__restrict__ logits, uint64_t pitch, uint64_t rows,
                                                                                 uint32_t vocab, uint32_t part_len, uint32_t parts,
@@ -128,46 +171,70 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void logprobs_kernel
                                                                                 typename stat_of<T>::type *ws, int32_t *ws_ids) {
     using A = typename stat_of<T>::type;
     constexpr int VE = 16 / sizeof(T);
-    constexpr int ROWS = WAVES == 1 ? 4 : 1; // rows of a work-group
+    constexpr int DEEP = sizeof(T) == 8 ? 2 : 4;
+    constexpr uint32_t CHUNK = WAVES * 64 * VE; // elements that the row's wavefronts load at once
+    constexpr int ROWS = WAVES == 1 ? 4 : 1;    // rows of a work-group
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const uint64_t unit = WAVES == 1 ? blockIdx.x * 4ull + wave : blockIdx.x;
+    const uint64_t unit = ROWS > 1 ? blockIdx.x * 4ull + wave : blockIdx.x;
     if (ROWS > 1 && unit >= rows * parts) return; // whole wavefronts; no barrier below with one wavefront to a row
-    const uint64_t row = parts == 1 ? unit : unit / parts;
+    const uint64_t row = parts == 1 ? unit : (uint32_t)unit / parts;
     const uint32_t part = parts == 1 ? 0 : (uint32_t)(unit - row * parts);
     const T *x = logits + row * pitch;
     const uint32_t begin = part * part_len, end = vocab - begin < part_len ? vocab : begin + part_len;
     Stats<A> st = no_stats<A>();
     Best<A> best{lowest(A(0)), -1};
-    A bar = lowest(A(0)); // the last of the list: only values above it enter
-    for (uint32_t c0 = begin + (WAVES == 1 ? 0 : wave * 64 * VE); c0 < end; c0 += WAVES * 64 * VE) {
-        const uint32_t c = c0 + lane * VE;
-        T raw[VE];
-        load_n<T, VE>(x + (c < end ? c : begin), c < end ? end - c : 0, raw);
-        A v[VE], cm;
+    A bar = lowest(A(0)); // only values above it enter the list
+    A floor = bar;        // the bar of the first step
+    for (uint32_t c0 = begin + (ROWS > 1 ? 0 : wave * 64 * VE); c0 < end; c0 += CHUNK * DEEP) {
+        T raw[DEEP][VE];
+        const uint32_t mine = c0 + lane * VE;
+        if (end - c0 >= CHUNK * (DEEP - 1) + 64 * VE) {
 #pragma unroll
-        for (int e = 0; e < VE; ++e) v[e] = (A)raw[e];
-        cm = v[0];
+            for (int u = 0; u < DEEP; ++u) __builtin_memcpy(raw[u], x + mine + u * CHUNK, 16);
+        } else {
 #pragma unroll
-        for (int e = 1; e < VE; ++e) cm = max_of(cm, v[e]);
+            for (int u = 0; u < DEEP; ++u) {
+                const uint32_t c = mine + u * CHUNK;
+                load_n<T, VE>(x + (c < end ? c : begin), c < end ? end - c : 0, raw[u]);
+            }
+        }
+        A cm = lowest(A(0));
+#pragma unroll
+        for (int u = 0; u < DEEP; ++u)
+#pragma unroll
+            for (int e = 0; e < VE; ++e) cm = max_of(cm, (A)raw[u][e]);
         if (cm > st.m) rebase(st, cm);
         const A m = st.m == lowest(A(0)) ? A(0) : st.m;
 #pragma unroll
-        for (int e = 0; e < VE; ++e) {
-            const A d = v[e] - m, p = exp_of(d);
-            st.s += p;
-            st.u += mul0(p, d);
-        }
-        if (TOP) {
-            uint64_t some = __ballot(cm > bar);
-            while (some) { // lanes in order, a lane's elements in order: equal values enter by index
-                const int l = __builtin_ctzll(some);
-                some &= some - 1;
+        for (int u = 0; u < DEEP; ++u)
 #pragma unroll
-                for (int e = 0; e < VE; ++e) {
-                    const A cand = __shfl(v[e], l);
-                    if (cand > bar) {
-                        insert(best, cand, (int32_t)(c0 + l * VE + e), lane);
-                        bar = __shfl(best.v, (int)top - 1);
+            for (int e = 0; e < VE; ++e) {
+                const A d = (A)raw[u][e] - m, p = exp_of(d);
+                st.s += p;
+                st.u += mul0(p, d);
+            }
+        if (TOP) {
+            if (c0 - begin < CHUNK) floor = bar = first_bar(cm, top, lane);
+            if (__ballot(cm > bar)) {
+#pragma unroll
+                for (int u = 0; u < DEEP; ++u) {
+                    uint32_t pass = 0;
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) pass |= (A)raw[u][e] > bar ? 1u << e : 0;
+                    uint64_t some = __ballot(pass != 0);
+                    while (some) { // lanes in order, a lane's elements in order: equal values enter by index
+                        const int l = __builtin_ctzll(some);
+                        some &= some - 1;
+                        const uint32_t bits = (uint32_t)lane_of((int)pass, l);
+#pragma unroll
+                        for (int e = 0; e < VE; ++e)
+                            if (bits >> e & 1) {
+                                const A cand = lane_of((A)raw[u][e], l);
+                                if (cand > bar) {
+                                    insert(best, cand, (int32_t)(c0 + u * CHUNK + l * VE + e), lane);
+                                    bar = max_of(lane_of(best.v, (int)top - 1), floor);
+                                }
+                            }
                     }
                 }
             }
@@ -216,7 +283,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void logprobs_kernel
                     const A q = bv[w * TOP_MAX + mid];
                     const int32_t qi = bi[w * TOP_MAX + mid];
                     // lists' unused ends are equal: by wavefront, so that every place is taken once
-                    const bool better = qi >= 0 ? (id < 0 || q > v || (q == v && qi < id)) : (id < 0 && (uint32_t)w < wave);
+                    const bool better = before(q, qi, v, id) || (qi < 0 && id < 0 && (uint32_t)w < wave);
                     if (better) lo = mid + 1;
                     else hi = mid;
                 }
@@ -234,7 +301,9 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void logprobs_kernel
     }
 }
 
-// Joins the parts of a row: one work-group of four wavefronts per row, a lane per candidate.
+// Joins the parts of a row, a work-group each.  With q = top / parts rounded up and r = top / q rounded up, the r-th best of
+// the parts' q-th alternatives has at least top - 1 others before it: it is a bar, and the few that are not behind it go to
+// LDS, where each counts those before it.
 template <typename T, bool TOP>
 __global__ __launch_bounds__(256) void logprobs_join_kernel(const T *__restrict__ logits, uint64_t pitch, uint64_t rows, uint32_t vocab,
                                                             uint32_t parts, uint32_t top, Outputs<typename stat_of<T>::type> o,
@@ -243,9 +312,18 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(const T *__restrict_
     const uint64_t row = blockIdx.x;
     const uint32_t lane = threadIdx.x % 64;
     Stats<A> st = no_stats<A>();
+    A bar = lowest(A(0));
+    int32_t bar_id = -1;
+    const A *v0 = ws + rows * parts * 3 + row * parts * top;
+    const int32_t *i0 = ws_ids + row * parts * top;
+    const uint32_t each = TOP ? (top + parts - 1) / parts : 1;
     if (lane < parts) { // at most 64 parts
         const A *p = ws + (row * parts + lane) * 3;
         st = {p[0], p[1], p[2]};
+        if (TOP) {
+            bar = v0[lane * top + each - 1];
+            bar_id = i0[lane * top + each - 1];
+        }
     }
 #pragma unroll
     for (int k = 32; k; k >>= 1) {
@@ -253,39 +331,52 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(const T *__restrict_
         st = join(st, other);
     }
     if (threadIdx.x == 0) finish_row<T, A>(o, logits + row * pitch, row, vocab, st);
-    if (TOP) {
-        const A *v0 = ws + rows * parts * 3 + row * parts * top;
-        const int32_t *i0 = ws_ids + row * parts * top;
+    if constexpr (TOP) {
+        __shared__ A cv[MAX_PARTS * TOP_MAX];
+        __shared__ int32_t ci[MAX_PARTS * TOP_MAX];
+        __shared__ uint32_t count;
+        if (threadIdx.x == 0) count = 0;
+        uint32_t above = 0;
+        for (uint32_t l = 0; l < parts; ++l) {
+            const int32_t id = lane_of(bar_id, l);
+            above += before(lane_of(bar, l), id, bar, bar_id) || (id < 0 && bar_id < 0 && l < lane);
+        }
+        const uint64_t at_bar = __ballot(lane < parts && above == (top + each - 1) / each - 1);
+        bar_id = lane_of(bar_id, __builtin_ctzll(at_bar));
+        bar = lane_of(bar, __builtin_ctzll(at_bar));
+        __syncthreads();
         for (uint32_t q = threadIdx.x; q < parts * top; q += 256) {
             const A v = v0[q];
             const int32_t id = i0[q];
-            const uint32_t mine = q / top;
-            uint32_t place = q - mine * top;
-            for (uint32_t w = 0; w < parts && place < top; ++w) {
-                if (w == mine) continue;
-                uint32_t lo = 0, hi = top;
-                while (lo < hi) {
-                    const uint32_t mid = (lo + hi) / 2;
-                    const A b = v0[w * top + mid];
-                    const int32_t bi = i0[w * top + mid];
-                    const bool better = bi >= 0 ? (id < 0 || b > v || (b == v && bi < id)) : (id < 0 && w < mine);
-                    if (better) lo = mid + 1;
-                    else hi = mid;
-                }
-                place += lo;
+            if (id >= 0 && !before(bar, bar_id, v, id)) { // (a part without so many alternatives: id < 0, no bar)
+                const uint32_t at = atomicAdd(&count, 1u); // any order: places are counted
+                cv[at] = v;
+                ci[at] = id;
             }
+        }
+        __syncthreads();
+        const uint32_t left = count;
+        for (uint32_t q = threadIdx.x; q < (left > top ? left : top); q += 256) {
+            if (q >= left) { // fewer alternatives than wanted
+                finish_top<A>(o, row, top, q, lowest(A(0)), -1, st);
+                continue;
+            }
+            const A v = cv[q];
+            const int32_t id = ci[q];
+            uint32_t place = 0;
+            for (uint32_t w = 0; w < left; ++w) place += before(cv[w], ci[w], v, id);
             if (place < top) finish_top<A>(o, row, top, place, v, id, st);
         }
     }
 }
 
-// Parts that a row is cut into, when the caller gives a workspace: so many that the launch has about two work-groups per
-// compute unit, each with at least 8192 elements.
+// Parts that a row is cut into, when the caller gives a workspace: so many that the launch has about four work-groups per
+// compute unit, each with at least 2048 elements.
 uint32_t row_parts(uint64_t rows, uint64_t vocab) {
-    if (rows >= 256) return 1;
-    uint64_t parts = (512 + rows - 1) / rows, most = vocab / 8192;
+    if (rows >= 1024) return 1;
+    uint64_t parts = (1024 + rows - 1) / rows, most = vocab / 2048;
     if (parts > most) parts = most;
-    if (parts > 64) parts = 64;
+    if (parts > MAX_PARTS) parts = MAX_PARTS;
     return parts < 2 ? 1 : (uint32_t)parts;
 }
 
@@ -335,22 +426,31 @@ int logprobs_launch(wk_stream *s, uint64_t rows, uint32_t vocab, const void *log
     return launch_status();
 }
 
+constexpr int GRAD_DEEP = 4;
+
 template <typename A> struct GradArgs {
     const A *lse, *entropy, *w, *h;
     const void *targets;
     bool wide_targets;
 };
 
-// One thread takes 16 bytes of a row; blockIdx.x counts a row's segments first.
+// One thread takes DEEP x 16 bytes of a row, all loads issued before any is used; blockIdx.x counts a row's segments first.
 template <typename T, bool ENTROPY>
 __global__ __launch_bounds__(256) void logprobs_grad_kernel(const T *x, uint64_t pitch, T *dx, uint64_t grad_pitch, uint32_t vocab,
                                                             uint32_t segments, GradArgs<typename stat_of<T>::type> a) {
     using A = typename stat_of<T>::type;
     constexpr int VE = 16 / sizeof(T);
-    const uint64_t row = blockIdx.x / segments;
-    const uint32_t seg = (uint32_t)(blockIdx.x - row * segments);
-    const uint32_t c = (seg * 256 + threadIdx.x) * VE;
-    if (c >= vocab) return;
+    const uint32_t row = blockIdx.x / segments;
+    const uint32_t seg = blockIdx.x - row * segments;
+    const uint32_t c0 = seg * (256 * VE * GRAD_DEEP) + threadIdx.x * VE;
+    const T *xr = x + (uint64_t)row * pitch;
+    T *dr = dx + (uint64_t)row * grad_pitch;
+    T raw[GRAD_DEEP][VE];
+#pragma unroll
+    for (int u = 0; u < GRAD_DEEP; ++u) {
+        const uint32_t c = c0 + u * 256 * VE;
+        load_n<T, VE>(xr + (c < vocab ? c : 0), c < vocab ? vocab - c : 0, raw[u]);
+    }
     const A lse = a.lse[row];
     A w = A(0), h = A(0), ent = A(0);
     int64_t t = -1;
@@ -363,30 +463,33 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(const T *x, uint64_t
         ent = a.entropy[row];
     }
     const bool empty = lse == lowest(A(0));
-    T raw[VE];
-    load_n<T, VE>(x + row * pitch + c, vocab - c, raw);
 #pragma unroll
-    for (int e = 0; e < VE; ++e) {
-        const A d = (A)raw[e] - lse, p = exp_of(d);
-        A g = -w * p;
-        if (ENTROPY) g -= h * mul0(p, d + ent);
-        if (t == (int64_t)(c + e)) g += w;
-        raw[e] = (T)(empty ? A(0) : g);
-    }
-    T *out = dx + row * grad_pitch + c;
-    if (vocab - c >= (uint32_t)VE) {
-        __builtin_memcpy(out, raw, sizeof raw);
-    } else {
+    for (int u = 0; u < GRAD_DEEP; ++u) {
+        const uint32_t c = c0 + u * 256 * VE;
+        if (c >= vocab) continue;
+        const bool here = t >= (int64_t)c && t < (int64_t)c + VE;
 #pragma unroll
-        for (int e = 0; e < VE; ++e)
-            if (c + e < vocab) out[e] = raw[e];
+        for (int e = 0; e < VE; ++e) {
+            const A d = (A)raw[u][e] - lse, p = exp_of(d);
+            A g = -w * p;
+            if (ENTROPY) g -= h * mul0(p, d + ent);
+            if (here && t == (int64_t)(c + e)) g += w;
+            raw[u][e] = (T)(empty ? A(0) : g);
+        }
+        if (vocab - c >= (uint32_t)VE) {
+            __builtin_memcpy(dr + c, raw[u], 16);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VE; ++e)
+                if (c + e < vocab) dr[c + e] = raw[u][e];
+        }
     }
 }
 
 template <typename T>
 int grad_launch(wk_stream *s, uint64_t rows, uint32_t vocab, const void *x, uint64_t pitch, void *dx, uint64_t grad_pitch,
                 const GradArgs<typename stat_of<T>::type> &a) {
-    constexpr uint32_t step = 256 * 16 / sizeof(T);
+    constexpr uint32_t step = 256 * GRAD_DEEP * 16 / sizeof(T);
     const uint32_t segments = (vocab + step - 1) / step;
     if (rows * segments > 0x7fffffffull) return WK_E_INVALID_VALUE;
     const dim3 grid((unsigned)(rows * segments));
