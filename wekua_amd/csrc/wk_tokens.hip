@@ -21,6 +21,7 @@ template <> struct stat_of<double> { using type = double; };
 constexpr uint32_t TOP_MAX = WK_TOKEN_TOP_MAX;
 static_assert(TOP_MAX == 64, "one alternative per lane");
 constexpr uint32_t MAX_PARTS = 64; // of a row: one per lane when they are joined
+constexpr int JOIN_THREADS = 1024;
 
 __device__ __forceinline__ float lowest(float) { return -__builtin_inff(); }
 __device__ __forceinline__ double lowest(double) { return -__builtin_inf(); }
@@ -64,12 +65,6 @@ __device__ __forceinline__ double lane_of(double v, int lane) {
 __device__ __forceinline__ int from_below(int v) { return __builtin_amdgcn_update_dpp(v, v, 0x138 /* wave_shr:1 */, 0xf, 0xf, false); }
 __device__ __forceinline__ float from_below(float v) { return __int_as_float(from_below(__float_as_int(v))); }
 __device__ __forceinline__ double from_below(double v) { return __hiloint2double(from_below(__double2hiint(v)), from_below(__double2loint(v))); }
-// the next value below a finite one; -inf stays
-__device__ __forceinline__ double just_below(double v) {
-    const long long b = __double_as_longlong(v);
-    return v == lowest(v) ? v : v == 0.0 ? __longlong_as_double((long long)0x8000000000000001ull) : __longlong_as_double(b > 0 ? b - 1 : b + 1);
-}
-
 // A wavefront's best values, lane l the l-th best with its index; lanes without one hold -inf and -1.
 template <typename A> struct Best {
     A v;
@@ -85,27 +80,25 @@ template <typename A> __device__ __forceinline__ void insert(Best<A> &b, A v, in
     b.id = lane > pos ? up_id : lane == pos ? id : b.id;
 }
 
-// A value that at least `top` of the wavefront's values are above, as high as it can be had cheaply: just below the top-th
-// largest of the lanes' maxima (-inf where so many lanes have none).  In f32 a lane's place is found by whole-number
-// comparisons of the value's order with the lane in its low six bits, which lowers the bar by up to 2^-16 of it.
-__device__ __forceinline__ float first_bar(float cm, uint32_t top, uint32_t lane) {
-    const uint32_t bits = __float_as_uint(cm);
-    const uint32_t order = (bits >> 31 ? ~bits : bits | 0x80000000u), key = (order & ~63u) | (63u - lane);
-    uint32_t above = 0;
-#pragma unroll 16
-    for (int l = 0; l < 64; ++l) above += (uint32_t)__builtin_amdgcn_readlane((int)key, l) > key;
-    const uint32_t k = (uint32_t)__builtin_amdgcn_readlane((int)(order & ~63u), __builtin_ctzll(__ballot(above == top - 1)));
-    const uint32_t low = k - 64; // a value before it (one step before +0 would be -0, its equal)
-    const float v = __uint_as_float(low >> 31 ? low & 0x7fffffffu : ~low);
+// A value that at least `top` of the wavefront's values are above: just below the top-th largest of the lanes' maxima, whose
+// order as a whole number is found bit by bit from above (20 bits; f64: of the upper word), one comparison of all lanes
+// each.  -inf where so many lanes have none.
+__device__ __forceinline__ uint32_t order_of(uint32_t bits) { return bits >> 31 ? ~bits : bits | 0x80000000u; }
+__device__ __forceinline__ uint32_t bar_order(uint32_t order, uint32_t top) {
+    uint32_t t = 0;
+#pragma unroll
+    for (uint32_t bit = 1u << 31; bit >= 1u << 12; bit >>= 1)
+        if ((uint32_t)__popcll(__ballot(order >= (t | bit))) >= top) t |= bit;
+    t -= 1u << 12; // a value before it (one step before +0 would be -0, its equal)
+    return t >> 31 ? t & 0x7fffffffu : ~t;
+}
+__device__ __forceinline__ float first_bar(float cm, uint32_t top) {
+    const float v = __uint_as_float(bar_order(order_of(__float_as_uint(cm)), top));
     return v == v ? v : lowest(v);
 }
-__device__ __forceinline__ double first_bar(double cm, uint32_t top, uint32_t lane) {
-    uint32_t above = 0;
-    for (int l = 0; l < 64; ++l) {
-        const double other = lane_of(cm, l);
-        above += other > cm || (other == cm && (uint32_t)l < lane);
-    }
-    return just_below(lane_of(cm, __builtin_ctzll(__ballot(above == top - 1))));
+__device__ __forceinline__ double first_bar(double cm, uint32_t top) {
+    const double v = __hiloint2double((int)bar_order(order_of((uint32_t)__double2hiint(cm)), top), 0);
+    return v == v ? v : lowest(v);
 }
 
 // whether (v, id) comes before (w, id_w) among the alternatives; id < 0: no value there, behind all others
@@ -120,6 +113,16 @@ template <typename T, int N> __device__ __forceinline__ void load_n(const T *p, 
 #pragma unroll
         for (int e = 0; e < N; ++e) raw[e] = (uint32_t)e < left ? p[e] : (T)-__builtin_inff();
     }
+}
+
+// `raw` was read at min(c, end - N): puts the elements from c on in front, -inf behind them.
+template <typename T, int N> __device__ __forceinline__ void raw_from_end(T raw[N], uint32_t c, uint32_t end) {
+    const uint32_t over = c <= end - N ? 0 : c - (end - N) < (uint32_t)N ? c - (end - N) : N; // elements of others in front
+    const T none = (T)-__builtin_inff();
+#pragma unroll
+    for (int s = N; s >= 1; s >>= 1)
+#pragma unroll
+        for (int e = 0; e < N; ++e) raw[e] = over & s ? (e + s < N ? raw[e + s] : none) : raw[e];
 }
 
 // What a row's finished statistics are written to; null pointers are not wanted.
@@ -188,9 +191,16 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void logprobs_kernel
     for (uint32_t c0 = begin + (ROWS > 1 ? 0 : wave * 64 * VE); c0 < end; c0 += CHUNK * DEEP) {
         T raw[DEEP][VE];
         const uint32_t mine = c0 + lane * VE;
-        if (end - c0 >= CHUNK * (DEEP - 1) + 64 * VE) {
+        const bool whole = end - c0 >= CHUNK * (DEEP - 1) + 64 * VE;
+        if (whole) {
 #pragma unroll
             for (int u = 0; u < DEEP; ++u) __builtin_memcpy(raw[u], x + mine + u * CHUNK, 16);
+        } else if (vocab >= VE) {
+            // the last 16 bytes in place of what reaches beyond them, then masked: nothing waits between the loads
+#pragma unroll
+            for (int u = 0; u < DEEP; ++u) __builtin_memcpy(raw[u], x + (mine + u * CHUNK <= end - VE ? mine + u * CHUNK : end - VE), 16);
+#pragma unroll
+            for (int u = 0; u < DEEP; ++u) raw_from_end<T, VE>(raw[u], mine + u * CHUNK, end);
         } else {
 #pragma unroll
             for (int u = 0; u < DEEP; ++u) {
@@ -198,11 +208,16 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void logprobs_kernel
                 load_n<T, VE>(x + (c < end ? c : begin), c < end ? end - c : 0, raw[u]);
             }
         }
-        A cm = lowest(A(0));
+        A cu[DEEP]; // the lane's maxima
 #pragma unroll
-        for (int u = 0; u < DEEP; ++u)
+        for (int u = 0; u < DEEP; ++u) {
+            cu[u] = (A)raw[u][0];
 #pragma unroll
-            for (int e = 0; e < VE; ++e) cm = max_of(cm, (A)raw[u][e]);
+            for (int e = 1; e < VE; ++e) cu[u] = max_of(cu[u], (A)raw[u][e]);
+        }
+        A cm = cu[0];
+#pragma unroll
+        for (int u = 1; u < DEEP; ++u) cm = max_of(cm, cu[u]);
         if (cm > st.m) rebase(st, cm);
         const A m = st.m == lowest(A(0)) ? A(0) : st.m;
 #pragma unroll
@@ -214,27 +229,20 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void logprobs_kernel
                 st.u += mul0(p, d);
             }
         if (TOP) {
-            if (c0 - begin < CHUNK) floor = bar = first_bar(cm, top, lane);
+            if (c0 - begin < CHUNK) floor = bar = first_bar(cm, top);
             if (__ballot(cm > bar)) {
 #pragma unroll
                 for (int u = 0; u < DEEP; ++u) {
-                    uint32_t pass = 0;
-#pragma unroll
-                    for (int e = 0; e < VE; ++e) pass |= (A)raw[u][e] > bar ? 1u << e : 0;
-                    uint64_t some = __ballot(pass != 0);
+                    uint64_t some = __ballot(cu[u] > bar);
                     while (some) { // lanes in order, a lane's elements in order: equal values enter by index
                         const int l = __builtin_ctzll(some);
                         some &= some - 1;
-                        const uint32_t bits = (uint32_t)lane_of((int)pass, l);
 #pragma unroll
-                        for (int e = 0; e < VE; ++e)
-                            if (bits >> e & 1) {
-                                const A cand = lane_of((A)raw[u][e], l);
-                                if (cand > bar) {
-                                    insert(best, cand, (int32_t)(c0 + u * CHUNK + l * VE + e), lane);
-                                    bar = max_of(lane_of(best.v, (int)top - 1), floor);
-                                }
-                            }
+                        for (int e = 0; e < VE; ++e) {
+                            if (!(__ballot((A)raw[u][e] > bar) >> l & 1)) continue;
+                            insert(best, lane_of((A)raw[u][e], l), (int32_t)(c0 + u * CHUNK + l * VE + e), lane);
+                            bar = max_of(lane_of(best.v, (int)top - 1), floor);
+                        }
                     }
                 }
             }
@@ -305,7 +313,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void logprobs_kernel
 // the parts' q-th alternatives has at least top - 1 others before it: it is a bar, and the few that are not behind it go to
 // LDS, where each counts those before it.
 template <typename T, bool TOP>
-__global__ __launch_bounds__(256) void logprobs_join_kernel(const T *__restrict__ logits, uint64_t pitch, uint64_t rows, uint32_t vocab,
+__global__ __launch_bounds__(JOIN_THREADS) void logprobs_join_kernel(const T *__restrict__ logits, uint64_t pitch, uint64_t rows, uint32_t vocab,
                                                             uint32_t parts, uint32_t top, Outputs<typename stat_of<T>::type> o,
                                                             const typename stat_of<T>::type *__restrict__ ws, const int32_t *__restrict__ ws_ids) {
     using A = typename stat_of<T>::type;
@@ -336,16 +344,16 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(const T *__restrict_
         __shared__ int32_t ci[MAX_PARTS * TOP_MAX];
         __shared__ uint32_t count;
         if (threadIdx.x == 0) count = 0;
-        uint32_t above = 0;
+        uint32_t above = 0; // parts are in the order of their indexes, and only a part without an alternative has -inf
         for (uint32_t l = 0; l < parts; ++l) {
-            const int32_t id = lane_of(bar_id, l);
-            above += before(lane_of(bar, l), id, bar, bar_id) || (id < 0 && bar_id < 0 && l < lane);
+            const A other = lane_of(bar, l);
+            above += other > bar || (other == bar && l < lane);
         }
         const uint64_t at_bar = __ballot(lane < parts && above == (top + each - 1) / each - 1);
         bar_id = lane_of(bar_id, __builtin_ctzll(at_bar));
         bar = lane_of(bar, __builtin_ctzll(at_bar));
         __syncthreads();
-        for (uint32_t q = threadIdx.x; q < parts * top; q += 256) {
+        for (uint32_t q = threadIdx.x; q < parts * top; q += JOIN_THREADS) {
             const A v = v0[q];
             const int32_t id = i0[q];
             if (id >= 0 && !before(bar, bar_id, v, id)) { // (a part without so many alternatives: id < 0, no bar)
@@ -356,7 +364,7 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(const T *__restrict_
         }
         __syncthreads();
         const uint32_t left = count;
-        for (uint32_t q = threadIdx.x; q < (left > top ? left : top); q += 256) {
+        for (uint32_t q = threadIdx.x; q < (left > top ? left : top); q += JOIN_THREADS) {
             if (q >= left) { // fewer alternatives than wanted
                 finish_top<A>(o, row, top, q, lowest(A(0)), -1, st);
                 continue;
@@ -419,9 +427,9 @@ int logprobs_launch(wk_stream *s, uint64_t rows, uint32_t vocab, const void *log
         const int rc = launch_status();
         if (rc) return rc;
         if (top)
-            hipLaunchKernelGGL((logprobs_join_kernel<T, true>), dim3((unsigned)rows), dim3(256), 0, s->stream, x, pitch, rows, vocab, parts, top, o, ws, ids);
+            hipLaunchKernelGGL((logprobs_join_kernel<T, true>), dim3((unsigned)rows), dim3(JOIN_THREADS), 0, s->stream, x, pitch, rows, vocab, parts, top, o, ws, ids);
         else
-            hipLaunchKernelGGL((logprobs_join_kernel<T, false>), dim3((unsigned)rows), dim3(256), 0, s->stream, x, pitch, rows, vocab, parts, top, o, ws, ids);
+            hipLaunchKernelGGL((logprobs_join_kernel<T, false>), dim3((unsigned)rows), dim3(64), 0, s->stream, x, pitch, rows, vocab, parts, top, o, ws, ids);
     }
     return launch_status();
 }
