@@ -21,7 +21,7 @@ template <> struct stat_of<double> { using type = double; };
 constexpr uint32_t TOP_MAX = WK_TOKEN_TOP_MAX;
 static_assert(TOP_MAX == 64, "one alternative per lane");
 constexpr uint32_t MAX_PARTS = 64; // of a row: one per lane when they are joined
-constexpr int JOIN_THREADS = 1024;
+constexpr int JOIN_WAVES = 16;
 
 __device__ __forceinline__ float lowest(float) { return -__builtin_inff(); }
 __device__ __forceinline__ double lowest(double) { return -__builtin_inf(); }
@@ -61,49 +61,89 @@ __device__ __forceinline__ float lane_of(float v, int lane) { return __int_as_fl
 __device__ __forceinline__ double lane_of(double v, int lane) {
     return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), lane), __builtin_amdgcn_readlane(__double2loint(v), lane));
 }
-// each lane's lower neighbour's value (lane 0: its own)
-__device__ __forceinline__ int from_below(int v) { return __builtin_amdgcn_update_dpp(v, v, 0x138 /* wave_shr:1 */, 0xf, 0xf, false); }
-__device__ __forceinline__ float from_below(float v) { return __int_as_float(from_below(__float_as_int(v))); }
-__device__ __forceinline__ double from_below(double v) { return __hiloint2double(from_below(__double2hiint(v)), from_below(__double2loint(v))); }
-// A wavefront's best values, lane l the l-th best with its index; lanes without one hold -inf and -1.
-template <typename A> struct Best {
+// the value of the lane whose number differs in the bit M, without a way through LDS
+template <int M> __device__ __forceinline__ int across(int v) {
+    if constexpr (M == 1) return __builtin_amdgcn_mov_dpp(v, 0xb1 /* quad_perm 1, 0, 3, 2 */, 0xf, 0xf, false);
+    if constexpr (M == 2) return __builtin_amdgcn_mov_dpp(v, 0x4e /* quad_perm 2, 3, 0, 1 */, 0xf, 0xf, false);
+    if constexpr (M == 4) { // groups of four: the even ones from four lanes up, the odd ones from four down
+        const int even = __builtin_amdgcn_update_dpp(v, v, 0x104 /* row_shl:4 */, 0xf, 0x5, false);
+        return __builtin_amdgcn_update_dpp(even, v, 0x114 /* row_shr:4 */, 0xf, 0xa, false);
+    }
+    if constexpr (M == 8) return __builtin_amdgcn_mov_dpp(v, 0x128 /* row_ror:8 */, 0xf, 0xf, false);
+    if constexpr (M == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+        return (int)(__lane_id() & 16 ? r[0] : r[1]);
+    }
+    if constexpr (M == 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+        return (int)(__lane_id() & 32 ? r[0] : r[1]);
+    }
+}
+template <int M> __device__ __forceinline__ float across(float v) { return __int_as_float(across<M>(__float_as_int(v))); }
+template <int M> __device__ __forceinline__ double across(double v) {
+    return __hiloint2double(across<M>(__double2hiint(v)), across<M>(__double2loint(v)));
+}
+
+// the statistics of all lanes, in each
+template <int M, typename A> __device__ __forceinline__ void join_lanes(Stats<A> &st) {
+    st = join(st, Stats<A>{across<M>(st.m), across<M>(st.s), across<M>(st.u)});
+    if constexpr (M > 1) join_lanes<M / 2>(st);
+}
+
+// Alternatives of a wavefront, one per lane: a value with its index.  Lanes without one hold -inf and NO_ID, which no masked logit
+// becomes: only values above -inf are ever taken.
+constexpr int32_t NO_ID = 0x7fffffff;
+template <typename A> struct Alt {
     A v;
     int32_t id;
 };
+template <typename A> __device__ __forceinline__ Alt<A> no_alt() { return {lowest(A(0)), NO_ID}; }
+template <typename A> __device__ __forceinline__ bool before(Alt<A> a, Alt<A> b) { return a.v > b.v || (a.v == b.v && a.id < b.id); }
 
-// Puts (v, id), the same in every lane and v > -inf, into the list, behind equal values that are in it already.
-template <typename A> __device__ __forceinline__ void insert(Best<A> &b, A v, int32_t id, uint32_t lane) {
-    const uint32_t pos = (uint32_t)__popcll(__ballot(b.v >= v));
-    const A up = from_below(b.v);
-    const int32_t up_id = from_below(b.id);
-    b.v = lane > pos ? up : lane == pos ? v : b.v;
-    b.id = lane > pos ? up_id : lane == pos ? id : b.id;
+// one step of a bitonic network: of the pair of lanes that differ in M, `best` lanes keep what comes first
+template <int M, typename A> __device__ __forceinline__ void exchange(Alt<A> &a, bool best) {
+    const Alt<A> o{across<M>(a.v), across<M>(a.id)};
+    if (before(o, a) == best) a = o;
+}
+template <int M, typename A> __device__ __forceinline__ void exchange_down(Alt<A> &a, uint32_t lane, bool first) {
+    exchange<M>(a, ((lane & M) == 0) == first);
+    if constexpr (M > 1) exchange_down<M / 2>(a, lane, first);
+}
+// the first 64 of two sorted lists, sorted: `b` comes in reverse
+template <typename A> __device__ __forceinline__ void merge_reversed(Alt<A> &a, Alt<A> b, uint32_t lane) {
+    if (before(b, a)) a = b;
+    exchange_down<32>(a, lane, true);
+}
+// a and a list in any order
+template <typename A> __device__ __forceinline__ void merge_unsorted(Alt<A> &a, Alt<A> b, uint32_t lane) {
+    exchange_down<1>(b, lane, (lane & 2) == 0);
+    exchange_down<2>(b, lane, (lane & 4) == 0);
+    exchange_down<4>(b, lane, (lane & 8) == 0);
+    exchange_down<8>(b, lane, (lane & 16) == 0);
+    exchange_down<16>(b, lane, (lane & 32) == 0);
+    exchange_down<32>(b, lane, false);
+    merge_reversed(a, b, lane);
 }
 
-// A value that at least `top` of the wavefront's values are above: just below the top-th largest of the lanes' maxima, whose
-// order as a whole number is found bit by bit from above (20 bits; f64: of the upper word), one comparison of all lanes
-// each.  -inf where so many lanes have none.
-__device__ __forceinline__ uint32_t order_of(uint32_t bits) { return bits >> 31 ? ~bits : bits | 0x80000000u; }
-__device__ __forceinline__ uint32_t bar_order(uint32_t order, uint32_t top) {
-    uint32_t t = 0;
+// Values in order as whole numbers, and back; what lies two below a value's number (one below +0 is -0, its equal) is less.
+__device__ __forceinline__ uint32_t order_of(float v) {
+    const uint32_t b = __float_as_uint(v);
+    return b >> 31 ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t order_of(double v) {
+    const uint64_t b = (uint64_t)__double_as_longlong(v);
+    return b >> 63 ? ~b : b | 0x8000000000000000ull;
+}
+__device__ __forceinline__ float value_of(uint32_t o) { return __uint_as_float(o >> 31 ? o & 0x7fffffffu : ~o); }
+__device__ __forceinline__ double value_of(uint64_t o) { return __longlong_as_double((long long)(o >> 63 ? o & 0x7fffffffffffffffull : ~o)); }
+
+// The top-th largest of the lanes' values, found bit by bit with one comparison of all lanes each.
+template <typename O> __device__ __forceinline__ O nth_order(O order, uint32_t top) {
+    O t = 0;
 #pragma unroll
-    for (uint32_t bit = 1u << 31; bit >= 1u << 12; bit >>= 1)
+    for (O bit = O(1) << (8 * sizeof(O) - 1); bit; bit >>= 1)
         if ((uint32_t)__popcll(__ballot(order >= (t | bit))) >= top) t |= bit;
-    t -= 1u << 12; // a value before it (one step before +0 would be -0, its equal)
-    return t >> 31 ? t & 0x7fffffffu : ~t;
-}
-__device__ __forceinline__ float first_bar(float cm, uint32_t top) {
-    const float v = __uint_as_float(bar_order(order_of(__float_as_uint(cm)), top));
-    return v == v ? v : lowest(v);
-}
-__device__ __forceinline__ double first_bar(double cm, uint32_t top) {
-    const double v = __hiloint2double((int)bar_order(order_of((uint32_t)__double2hiint(cm)), top), 0);
-    return v == v ? v : lowest(v);
-}
-
-// whether (v, id) comes before (w, id_w) among the alternatives; id < 0: no value there, behind all others
-template <typename A> __device__ __forceinline__ bool before(A v, int32_t id, A w, int32_t id_w) {
-    return id >= 0 && (id_w < 0 || v > w || (v == w && id < id_w));
+    return t;
 }
 
 template <typename T, int N> __device__ __forceinline__ void load_n(const T *p, uint32_t left, T raw[N]) {
@@ -154,19 +194,22 @@ __device__ __forceinline__ void finish_row(const Outputs<A> &o, const T *x, uint
     }
 }
 
-template <typename A> __device__ __forceinline__ void finish_top(const Outputs<A> &o, uint64_t row, uint32_t top, uint32_t place, A v, int32_t id, Stats<A> st) {
+template <typename A> __device__ __forceinline__ void finish_top(const Outputs<A> &o, uint64_t row, uint32_t top, uint32_t place, Alt<A> a, Stats<A> st) {
     const bool bad = !(st.s < A(__builtin_inff()));
-    const bool none = bad || !(v > lowest(A(0)));
-    o.top_ids[row * top + place] = none ? -1 : id;
-    o.top_logprobs[row * top + place] = bad ? A(__builtin_nanf("")) : none ? lowest(A(0)) : (v - st.m) - log(st.s);
+    const bool none = bad || a.id == NO_ID;
+    o.top_ids[row * top + place] = none ? -1 : a.id;
+    o.top_logprobs[row * top + place] = bad ? A(__builtin_nanf("")) : none ? lowest(A(0)) : (a.v - st.m) - log(st.s);
 }
 
 // One row, or a part of one, over the 64 * WAVES threads of a work-group (WAVES = 1: four rows to a work-group).  A part
 // leaves its statistics and its alternatives in `ws`; a whole row is finished here.
 //
-// A lane takes DEEP x 16 bytes a step, all loads issued before any is used.  An alternative enters the list in ~100 cycles of the
-// whole wavefront, so few should: in the first step the top-th largest of the lanes' maxima is already a bar
-// under which nothing can be among the best (at least `top` values reach it), afterwards the list's last value is.
+// A lane takes DEEP x 16 bytes a step, all loads issued before any is used.  Alternatives: the top-th largest of the lanes' running
+// maxima is a value t that the wavefront has seen `top` times or more.  In the step that brings it, only elements not below
+// t can be among the best, in later steps (higher indexes) only elements above it; those few are collected in LDS.  Where 64 come
+// together they are sorted over the lanes and merged with the best so far; most rows get there once, at their end, with what all
+// their wavefronts have collected.  (Putting alternatives into a sorted list one by one cost 0.25 us each where a
+// wavefront has a unit for itself: one row of 131072, 64 alternatives 28 us for its parts.)
 template <typename T, int WAVES, bool TOP>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void logprobs_kernel(const T *__restrict__ logits, uint64_t pitch, uint64_t rows,
                                                                                 uint32_t vocab, uint32_t part_len, uint32_t parts,
@@ -185,9 +228,30 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void logprobs_kernel
     const T *x = logits + row * pitch;
     const uint32_t begin = part * part_len, end = vocab - begin < part_len ? vocab : begin + part_len;
     Stats<A> st = no_stats<A>();
-    Best<A> best{lowest(A(0)), -1};
-    A bar = lowest(A(0)); // only values above it enter the list
-    A floor = bar;        // the bar of the first step
+    Alt<A> best = no_alt<A>();
+    A bar = lowest(A(0)); // only values above it are collected
+    constexpr int LISTS = TOP ? WAVES * ROWS : 1;
+    __shared__ A lv[LISTS][TOP ? 2 * TOP_MAX : 1]; // a wavefront's collection
+    __shared__ int32_t li[LISTS][TOP ? 2 * TOP_MAX : 1];
+    uint32_t held = 0, taken = 0; // in the collection; since the bar moved
+    bool sorted = false; // there is something in `best`
+    // takes the first 64 of the collection into the best
+    auto absorb = [&]() {
+        const uint32_t n = held < 64 ? held : 64;
+        Alt<A> b = no_alt<A>();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); // other lanes wrote it: nothing read before may stand for it
+        if (lane < n) b = {lv[wave][lane], li[wave][lane]};
+        const bool rest = lane + 64 < held;
+        const Alt<A> r{rest ? lv[wave][lane + 64] : A(0), rest ? li[wave][lane + 64] : 0};
+        merge_unsorted(best, b, lane);
+        if (rest) {
+            lv[wave][lane] = r.v;
+            li[wave][lane] = r.id;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        held -= n;
+        sorted = true;
+    };
     for (uint32_t c0 = begin + (ROWS > 1 ? 0 : wave * 64 * VE); c0 < end; c0 += CHUNK * DEEP) {
         T raw[DEEP][VE];
         const uint32_t mine = c0 + lane * VE;
@@ -229,44 +293,56 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void logprobs_kernel
                 st.u += mul0(p, d);
             }
         if (TOP) {
-            if (c0 - begin < CHUNK) floor = bar = first_bar(cm, top);
             if (__ballot(cm > bar)) {
+                // the bar moves in the first step and after every twelve that came over it
+                A seen = bar, gate = bar;
+                if (c0 - begin < CHUNK || taken >= 12) {
+                    const auto nth = nth_order(order_of(st.m), top);
+                    const A under = value_of(nth - 2); // (NaN below -inf)
+                    seen = value_of(nth);
+                    if (under > bar) gate = under;
+                    taken = 0;
+                }
 #pragma unroll
                 for (int u = 0; u < DEEP; ++u) {
-                    uint64_t some = __ballot(cu[u] > bar);
-                    while (some) { // lanes in order, a lane's elements in order: equal values enter by index
-                        const int l = __builtin_ctzll(some);
-                        some &= some - 1;
+                    if (!__ballot(cu[u] > gate)) continue;
 #pragma unroll
-                        for (int e = 0; e < VE; ++e) {
-                            if (!(__ballot((A)raw[u][e] > bar) >> l & 1)) continue;
-                            insert(best, lane_of((A)raw[u][e], l), (int32_t)(c0 + u * CHUNK + l * VE + e), lane);
-                            bar = max_of(lane_of(best.v, (int)top - 1), floor);
+                    for (int e = 0; e < VE; ++e) {
+                        const A v = (A)raw[u][e];
+                        const uint64_t some = __ballot(v > gate);
+                        if (!some) continue;
+                        if (v > gate) {
+                            const uint32_t at = held + __builtin_amdgcn_mbcnt_hi((uint32_t)(some >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)some, 0));
+                            lv[wave][at] = v;
+                            li[wave][at] = (int32_t)(mine + u * CHUNK + e);
                         }
+                        held += (uint32_t)__popcll(some);
+                        taken += (uint32_t)__popcll(some);
+                        if (held >= 64) absorb();
                     }
                 }
+                bar = seen;
             }
         }
     }
-#pragma unroll
-    for (int k = 32; k; k >>= 1) {
-        Stats<A> other{__shfl_xor(st.m, k), __shfl_xor(st.s, k), __shfl_xor(st.u, k)};
-        st = join(st, other);
-    }
+    if (TOP && ROWS > 1 && held) absorb();
+    join_lanes<32>(st);
     if constexpr (WAVES == 1) {
         if (parts == 1) {
             if (lane == 0) finish_row<T, A>(o, x, row, vocab, st);
-            if (TOP && lane < top) finish_top<A>(o, row, top, lane, best.v, best.id, st);
+            if (TOP && lane < top) finish_top<A>(o, row, top, lane, best, st);
         }
     } else {
         __shared__ Stats<A> all[WAVES];
-        __shared__ A bv[TOP ? WAVES * TOP_MAX : 1];
-        __shared__ int32_t bi[TOP ? WAVES * TOP_MAX : 1];
-        if (lane == 0) all[wave] = st;
-        if (TOP && lane < top) {
-            bv[wave * TOP_MAX + lane] = best.v;
-            bi[wave * TOP_MAX + lane] = best.id;
+        __shared__ A bars[WAVES];
+        __shared__ A tv[TOP ? WAVES * 64 : 1]; // what is left of all wavefronts' collections
+        __shared__ int32_t ti[TOP ? WAVES * 64 : 1];
+        __shared__ uint32_t total;
+        if (lane == 0) {
+            all[wave] = st;
+            if (TOP) bars[wave] = bar;
         }
+        if (TOP && threadIdx.x == 0) total = 0;
         __syncthreads();
         st = all[0];
 #pragma unroll
@@ -278,103 +354,94 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void logprobs_kernel
             ws[unit * 3 + 1] = st.s;
             ws[unit * 3 + 2] = st.u;
         }
-        if (TOP && lane < top) {
-            // place among all lists: the own one's elements in front, and what the others have that is better
-            const A v = best.v;
-            const int32_t id = best.id;
-            uint32_t place = lane;
-            for (int w = 0; w < WAVES; ++w) {
-                if ((uint32_t)w == wave) continue;
-                uint32_t lo = 0, hi = top; // the first entry that is not better
-                while (lo < hi) {
-                    const uint32_t mid = (lo + hi) / 2;
-                    const A q = bv[w * TOP_MAX + mid];
-                    const int32_t qi = bi[w * TOP_MAX + mid];
-                    // lists' unused ends are equal: by wavefront, so that every place is taken once
-                    const bool better = before(q, qi, v, id) || (qi < 0 && id < 0 && (uint32_t)w < wave);
-                    if (better) lo = mid + 1;
-                    else hi = mid;
-                }
-                place += lo;
+        if constexpr (TOP) {
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) bar = max_of(bar, bars[w]); // what any of them has seen `top` times
+            const Alt<A> c = lane < held ? Alt<A>{lv[wave][lane], li[wave][lane]} : no_alt<A>();
+            const bool stays = lane < held && c.v >= bar;
+            const uint64_t some = __ballot(stays);
+            uint32_t base = 0;
+            if (lane == 0 && some) base = atomicAdd(&total, (uint32_t)__popcll(some)); // in any order: they are sorted
+            base = (uint32_t)lane_of((int)base, 0);
+            if (stays) {
+                const uint32_t at = base + __builtin_amdgcn_mbcnt_hi((uint32_t)(some >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)some, 0));
+                tv[at] = c.v;
+                ti[at] = c.id;
             }
-            if (place < top) {
-                if (parts == 1) {
-                    finish_top<A>(o, row, top, place, v, id, st);
-                } else {
-                    ws[rows * parts * 3 + unit * top + place] = v;
-                    ws_ids[unit * top + place] = id;
+            if (sorted && wave) {
+                lv[wave][127 - lane] = best.v; // in reverse, behind the collection
+                li[wave][127 - lane] = best.id;
+            }
+            __shared__ uint32_t has_list[WAVES];
+            if (lane == 0) has_list[wave] = sorted;
+            __syncthreads();
+            if (wave == 0) {
+                for (uint32_t q = 0; q < total; q += 64) {
+                    const Alt<A> b = q + lane < total ? Alt<A>{tv[q + lane], ti[q + lane]} : no_alt<A>();
+                    merge_unsorted(best, b, lane);
+                }
+                for (int w = 1; w < WAVES; ++w)
+                    if (has_list[w]) merge_reversed(best, Alt<A>{lv[w][64 + lane], li[w][64 + lane]}, lane);
+                if (lane < top) {
+                    if (parts == 1) {
+                        finish_top<A>(o, row, top, lane, best, st);
+                    } else {
+                        ws[rows * parts * 3 + unit * top + lane] = best.v;
+                        ws_ids[unit * top + lane] = best.id;
+                    }
                 }
             }
         }
     }
 }
 
-// Joins the parts of a row, a work-group each.  With q = top / parts rounded up and r = top / q rounded up, the r-th best of
-// the parts' q-th alternatives has at least top - 1 others before it: it is a bar, and the few that are not behind it go to
-// LDS, where each counts those before it.
+// Joins the parts of a row, a work-group each: sixteen wavefronts merge up to four lists each, then each other's.
 template <typename T, bool TOP>
-__global__ __launch_bounds__(JOIN_THREADS) void logprobs_join_kernel(const T *__restrict__ logits, uint64_t pitch, uint64_t rows, uint32_t vocab,
-                                                            uint32_t parts, uint32_t top, Outputs<typename stat_of<T>::type> o,
-                                                            const typename stat_of<T>::type *__restrict__ ws, const int32_t *__restrict__ ws_ids) {
+__global__ __launch_bounds__(TOP ? JOIN_WAVES * 64 : 64) void logprobs_join_kernel(const T *__restrict__ logits, uint64_t pitch, uint64_t rows, uint32_t vocab,
+                                                                                   uint32_t parts, uint32_t top, Outputs<typename stat_of<T>::type> o,
+                                                                                   const typename stat_of<T>::type *__restrict__ ws, const int32_t *__restrict__ ws_ids) {
     using A = typename stat_of<T>::type;
     const uint64_t row = blockIdx.x;
-    const uint32_t lane = threadIdx.x % 64;
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    constexpr int LISTS = MAX_PARTS / JOIN_WAVES;
     Stats<A> st = no_stats<A>();
-    A bar = lowest(A(0));
-    int32_t bar_id = -1;
-    const A *v0 = ws + rows * parts * 3 + row * parts * top;
-    const int32_t *i0 = ws_ids + row * parts * top;
-    const uint32_t each = TOP ? (top + parts - 1) / parts : 1;
-    if (lane < parts) { // at most 64 parts
+    if (lane < parts && wave == 0) {
         const A *p = ws + (row * parts + lane) * 3;
         st = {p[0], p[1], p[2]};
-        if (TOP) {
-            bar = v0[lane * top + each - 1];
-            bar_id = i0[lane * top + each - 1];
-        }
     }
+    Alt<A> list[LISTS];
+    if (TOP) {
+        const A *v0 = ws + rows * parts * 3 + row * parts * top;
+        const int32_t *i0 = ws_ids + row * parts * top;
 #pragma unroll
-    for (int k = 32; k; k >>= 1) {
-        Stats<A> other{__shfl_xor(st.m, k), __shfl_xor(st.s, k), __shfl_xor(st.u, k)};
-        st = join(st, other);
+        for (int k = 0; k < LISTS; ++k) { // the first one forwards, the others in reverse
+            const uint32_t p = wave + k * JOIN_WAVES, at = k ? 63 - lane : lane;
+            list[k] = no_alt<A>();
+            if (p < parts && at < top) list[k] = {v0[p * top + at], i0[p * top + at]};
+        }
     }
-    if (threadIdx.x == 0) finish_row<T, A>(o, logits + row * pitch, row, vocab, st);
+    if (wave == 0) {
+        join_lanes<32>(st);
+        if (lane == 0) finish_row<T, A>(o, logits + row * pitch, row, vocab, st);
+    }
     if constexpr (TOP) {
-        __shared__ A cv[MAX_PARTS * TOP_MAX];
-        __shared__ int32_t ci[MAX_PARTS * TOP_MAX];
-        __shared__ uint32_t count;
-        if (threadIdx.x == 0) count = 0;
-        uint32_t above = 0; // parts are in the order of their indexes, and only a part without an alternative has -inf
-        for (uint32_t l = 0; l < parts; ++l) {
-            const A other = lane_of(bar, l);
-            above += other > bar || (other == bar && l < lane);
-        }
-        const uint64_t at_bar = __ballot(lane < parts && above == (top + each - 1) / each - 1);
-        bar_id = lane_of(bar_id, __builtin_ctzll(at_bar));
-        bar = lane_of(bar, __builtin_ctzll(at_bar));
-        __syncthreads();
-        for (uint32_t q = threadIdx.x; q < parts * top; q += JOIN_THREADS) {
-            const A v = v0[q];
-            const int32_t id = i0[q];
-            if (id >= 0 && !before(bar, bar_id, v, id)) { // (a part without so many alternatives: id < 0, no bar)
-                const uint32_t at = atomicAdd(&count, 1u); // any order: places are counted
-                cv[at] = v;
-                ci[at] = id;
+        __shared__ A lv[JOIN_WAVES][64];
+        __shared__ int32_t li[JOIN_WAVES][64];
+#pragma unroll
+        for (int k = 1; k < LISTS; ++k)
+            if (wave + k * JOIN_WAVES < parts) merge_reversed(list[0], list[k], lane);
+        uint32_t left = parts < JOIN_WAVES ? parts : JOIN_WAVES; // wavefronts with a list
+        while (left > 1) {
+            const uint32_t half = (left + 1) / 2;
+            if (wave >= half && wave < left) {
+                lv[wave][63 - lane] = list[0].v;
+                li[wave][63 - lane] = list[0].id;
             }
+            __syncthreads();
+            if (wave + half < left) merge_reversed(list[0], Alt<A>{lv[wave + half][lane], li[wave + half][lane]}, lane);
+            left = half;
         }
-        __syncthreads();
-        const uint32_t left = count;
-        for (uint32_t q = threadIdx.x; q < (left > top ? left : top); q += JOIN_THREADS) {
-            if (q >= left) { // fewer alternatives than wanted
-                finish_top<A>(o, row, top, q, lowest(A(0)), -1, st);
-                continue;
-            }
-            const A v = cv[q];
-            const int32_t id = ci[q];
-            uint32_t place = 0;
-            for (uint32_t w = 0; w < left; ++w) place += before(cv[w], ci[w], v, id);
-            if (place < top) finish_top<A>(o, row, top, place, v, id, st);
-        }
+        if (wave == 0 && lane < top) finish_top<A>(o, row, top, lane, list[0], st);
     }
 }
 
@@ -427,7 +494,7 @@ int logprobs_launch(wk_stream *s, uint64_t rows, uint32_t vocab, const void *log
         const int rc = launch_status();
         if (rc) return rc;
         if (top)
-            hipLaunchKernelGGL((logprobs_join_kernel<T, true>), dim3((unsigned)rows), dim3(JOIN_THREADS), 0, s->stream, x, pitch, rows, vocab, parts, top, o, ws, ids);
+            hipLaunchKernelGGL((logprobs_join_kernel<T, true>), dim3((unsigned)rows), dim3(JOIN_WAVES * 64), 0, s->stream, x, pitch, rows, vocab, parts, top, o, ws, ids);
         else
             hipLaunchKernelGGL((logprobs_join_kernel<T, false>), dim3((unsigned)rows), dim3(64), 0, s->stream, x, pitch, rows, vocab, parts, top, o, ws, ids);
     }
