@@ -188,7 +188,100 @@ template <bool ALIGNED, typename O> __global__ __launch_bounds__(256) void gemm_
         for (int j = 0; j < 4; ++j) store_row4<O>(a, m0 + wm + 16 * i + r16, n0 + wn + 16 * j + 4 * g, acc[i][j]);
 }
 
+// Few rows: 16 MT rows of A against 16 NT rows of B, which is streamed once from memory straight into the lanes' operand
+// registers (both operands assign k to lanes alike, and a sum does not care which k that is).  The eight wavefronts of a
+// work-group take every eighth block of k, DEEP of them in flight each, and their sums meet in LDS in wavefront order.
+template <bool ALIGNED, typename O, int MT, int NT, int DEEP> __global__ __launch_bounds__(512) void gemm_f8_rows_kernel(F8Args a) {
+    constexpr uint32_t WAVES = 8;
+    __shared__ f32x4 part[WAVES][MT * NT][64];
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, r16 = lane % 16, g = lane / 16;
+    const uint32_t n0 = blockIdx.x * (16 * NT), m0 = blockIdx.y * (16 * MT);
+    const uint8_t *pa[MT], *pb[NT];
+    const float *psa[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const uint32_t m = m0 + 16 * i + r16, row = m < a.M ? m : a.M - 1;
+        pa[i] = a.A + (uint64_t)row * a.lda;
+        psa[i] = a.sa + (uint64_t)row * a.sap;
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const uint32_t n = n0 + 16 * j + r16;
+        pb[j] = a.B + (uint64_t)(n < a.N ? n : a.N - 1) * a.ldb;
+    }
+    const float *psb = a.sb + (uint64_t)(n0 / KB) * a.sbp; // 16 NT divides 128: one row of scales
+    f32x4 acc[MT][NT] = {};
+    const uint32_t whole = a.K / KB; // blocks that need no look at K
+    i32x4 ca[DEEP][MT][2], cb[DEEP][NT][2];
+    float sa[DEEP][MT], sb[DEEP];
+    auto fetch = [&](int d, uint32_t kb, bool inside) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t k = kb * KB + h * 64 + g * 16;
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+                cb[d][j][h] = inside && ALIGNED ? *reinterpret_cast<const i32x4 *>(pb[j] + k) : load_chunk<ALIGNED>(pb[j], k, a.K);
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+                ca[d][i][h] = inside && ALIGNED ? *reinterpret_cast<const i32x4 *>(pa[i] + k) : load_chunk<ALIGNED>(pa[i], k, a.K);
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) sa[d][i] = psa[i][kb];
+        sb[d] = psb[kb];
+    };
+    auto multiply = [&](int d) {
+        Wide wb[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) wb[j] = widen_codes(__builtin_shufflevector(cb[d][j][0], cb[d][j][1], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const Wide wa = widen_codes(__builtin_shufflevector(ca[d][i][0], ca[d][i][1], 0, 1, 2, 3, 4, 5, 6, 7));
+            const float s = sa[d][i] * sb[d];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const f32x4 p = mfma_block(wb[j], wa, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(p[e], s, acc[i][j][e]);
+            }
+        }
+    };
+    uint32_t kb = wave;
+    for (; kb + (DEEP - 1) * WAVES < whole; kb += DEEP * WAVES) {
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d) fetch(d, kb + d * WAVES, true);
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d) multiply(d);
+    }
+    for (; kb < a.kblocks; kb += WAVES) {
+        fetch(0, kb, kb < whole);
+        multiply(0);
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) part[wave][i * NT + j][lane] = acc[i][j];
+    __syncthreads();
+    for (uint32_t t = wave; t < MT * NT; t += WAVES) {
+        f32x4 sum = part[0][t][lane];
+#pragma unroll
+        for (uint32_t w = 1; w < WAVES; ++w) sum += part[w][t][lane];
+        store_row4<O>(a, m0 + 16 * (t / NT) + r16, n0 + 16 * (t % NT) + 4 * g, sum);
+    }
+}
+
+template <bool ALIGNED, typename O> int gemm_f8_rows_launch(hipStream_t st, const F8Args &a) {
+    const dim3 block(512);
+    if (a.M <= 16)
+        hipLaunchKernelGGL((gemm_f8_rows_kernel<ALIGNED, O, 1, 1, 4>), dim3((a.N + 15) / 16), block, 0, st, a);
+    else if (a.M <= 32)
+        hipLaunchKernelGGL((gemm_f8_rows_kernel<ALIGNED, O, 2, 1, 4>), dim3((a.N + 15) / 16), block, 0, st, a);
+    else
+        hipLaunchKernelGGL((gemm_f8_rows_kernel<ALIGNED, O, 4, 1, 2>), dim3((a.N + 15) / 16, (a.M + 63) / 64), block, 0, st, a);
+    return launch_status();
+}
+
 template <typename O> int gemm_f8_launch(wk_stream *s, const F8Args &a, bool aligned) {
+    if (a.M <= 64) return aligned ? gemm_f8_rows_launch<true, O>(s->stream, a) : gemm_f8_rows_launch<false, O>(s->stream, a);
     const uint64_t tiles = (uint64_t)((a.M + 127) / 128) * ((a.N + 127) / 128);
     if (tiles > 0x7fffffffull) return WK_E_INVALID_VALUE;
     if (aligned)
