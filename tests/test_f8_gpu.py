@@ -69,7 +69,7 @@ def test_quantize_extremes(dev, block_rows):
         b.free()
 
 
-def check_gemm(dev, M, N, K, out="f32", bias=False, kind=-1, pads=(0, 0, 0), shift=0, seed=0, codes=None):
+def check_gemm(dev, M, N, K, out="f32", bias=False, kind=-1, pads=(0, 0, 0), shift=0, seed=0, codes=None, cut=True):
     rng = np.random.RandomState(seed + M * 7 + N * 3 + K)
     kb = -(-K // 128)
     a = codes(rng, M, K) if codes else ot.e4m3_encode(np.clip(rng.randn(M, K) * 60, -448, 448))
@@ -88,7 +88,7 @@ def check_gemm(dev, M, N, K, out="f32", bias=False, kind=-1, pads=(0, 0, 0), shi
     got = bc.download(poison.dtype, (M, ldc))
     assert (got[:, N:] == poison).all(), "wrote outside C"
     got = values(out, got[:, :N])
-    want, mag, largest = ot.gemm_f8(a, sa, b, sb, bi, kind)
+    want, mag, largest = ot.gemm_f8(a, sa, b, sb, bi, kind, cut)
     tol = (128 + kb + 2) * 2.0 ** -23 * mag + (2.0 ** -23 * (np.abs(want) + mag) if bias else 0)
     tol += 7 * 2.0 ** -13 * largest if out != "f32" else 0
     tol += (2.0 ** -20 if kind >= 0 else 0) + {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}[out] * np.abs(want) * 1.01
@@ -106,6 +106,14 @@ def test_gemm_sizes(dev, M, N, K):
     """Rows on 16-byte boundaries behind a gap, and rows that follow each other at whatever K is."""
     check_gemm(dev, M, N, K, pads=(-K % 16, -K % 16 + 16, 3))
     check_gemm(dev, M, N, K, pads=(1 if K % 16 == 0 else 0, 0, 0))
+
+
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("M,N,K,kind", [(65, 16, 128, -1), (2048, 192, 1100, 1), (3600, 3700, 136, -1), (3840, 3584, 640, -1), (3601, 3900, 1280, 0), (1, 20000, 512, -1)])
+def test_gemm_large(dev, out, M, N, K, kind):
+    """Every tile size, whole tiles and ragged ones, one to ten blocks of k with and without a short one behind them, against a
+    product in 64 bits; the eight products' largest is bounded by their sum."""
+    check_gemm(dev, M, N, K, out, kind == 0, kind, pads=(-K % 16, -K % 16, 4 if M % 2 else 0), cut=False)
 
 
 @pytest.mark.parametrize("out", ["f32", "f16", "bf16"])

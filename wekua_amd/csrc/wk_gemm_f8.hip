@@ -12,6 +12,7 @@
 // The instruction gets B's rows as its first operand and A's as its second: a lane then holds four consecutive columns
 // of one row of C, so the scale of A is one value per lane and 16 rows, and C is stored four elements at a time.
 #include "wk_internal.hpp"
+#include "wk_lds_dma.hpp"
 
 #include <type_traits>
 
@@ -93,7 +94,7 @@ template <bool ALIGNED> __device__ __forceinline__ i32x4 load_chunk(const uint8_
     return v;
 }
 
-template <typename O> __device__ __forceinline__ void store_row4(const F8Args &a, uint32_t m, uint32_t n, f32x4 v) {
+template <typename O, bool ACT = true> __device__ __forceinline__ void store_row4(const F8Args &a, uint32_t m, uint32_t n, f32x4 v) {
     if (m >= a.M || n >= a.N) return;
     O *p = static_cast<O *>(a.C) + (uint64_t)m * a.ldc + n;
     O out[4];
@@ -102,7 +103,7 @@ template <typename O> __device__ __forceinline__ void store_row4(const F8Args &a
     for (int e = 0; e < 4; ++e) {
         float y = v[e];
         if (a.bias) y += a.bias[whole || n + e < a.N ? n + e : n];
-        out[e] = (O)act_forward<float>(a.kind, y);
+        out[e] = (O)(ACT ? act_forward<float>(a.kind, y) : y);
     }
     if (whole) {
         __builtin_memcpy(p, out, sizeof out);
@@ -186,6 +187,261 @@ template <bool ALIGNED, typename O> __global__ __launch_bounds__(256) void gemm_
     for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) store_row4<O>(a, m0 + wm + 16 * i + r16, n0 + wn + 16 * j + 4 * g, acc[i][j]);
+}
+
+// The kernel for aligned operands.  WM x WN wavefronts with 16 MT x 16 NT of C each; k-blocks go from memory straight into
+// LDS, two of them at a time in the two halves of it (rows and chunks as above, the swizzle on the source's side), the scales
+// with them.
+//
+// Per block a wavefront reads its NT operands of B once and its MT operands of A one ahead of use.  When the last of them
+// is in registers the wavefronts meet: the block is read, the next one has landed (it was asked for a whole block ago), the one after
+// that is asked for, and the next block's first operands are read while the last row of products still runs.
+template <typename O, int WM, int WN, int MT, int NT> struct DmaTile {
+    static constexpr uint32_t TM = WM * MT * 16, TN = WN * NT * 16, THREADS = WM * WN * 64;
+    static constexpr uint32_t NB = TN > KB ? TN / KB : 1; // rows of B's scales
+    static constexpr uint32_t A_BYTES = TM * KB, B_BYTES = TN * KB, SCALE_BYTES = WM * WN * 256; // (64 scales per wavefront)
+    static constexpr uint32_t HALF = A_BYTES + B_BYTES + SCALE_BYTES;
+    static_assert(TM % 64 == 0 && TM / 64 < WM * WN && A_BYTES % (16 * THREADS) == 0 && B_BYTES % (16 * THREADS) == 0 && NB <= 64);
+};
+
+// tile number -> its place: consecutive work-groups go to the eight dies in turn, so each die gets a run of its own, walked in groups
+// of eight rows of tiles: what a die multiplies at a time shares rows of A and B in its L2
+__device__ __forceinline__ void tile_place(uint32_t id, uint32_t tiles, uint32_t tiles_m, uint32_t tiles_n, uint32_t &tm, uint32_t &tn) {
+    const uint32_t die = id & 7, per = tiles >> 3, extra = tiles & 7;
+    const uint32_t t = die * per + (die < extra ? die : extra) + (id >> 3);
+    const uint32_t wide = 8 * tiles_n, group = t / wide, rest = t - group * wide;
+    const uint32_t rows = tiles_m - group * 8 < 8 ? tiles_m - group * 8 : 8;
+    tn = rest / rows;
+    tm = group * 8 + (rest - tn * rows);
+}
+
+// The direct loads of wk_lds_dma.hpp with five wait states in front: the compiler may form the scalar base in vector registers and
+// read it back (it does, for a block number that hangs on a comparison), a vector instruction that writes a scalar register
+// wants five before a memory instruction reads it, and inside inline assembly nobody else puts them there.
+__device__ __forceinline__ void load16(const void *base, uint32_t byte_offset, uint32_t lds_base) {
+    asm volatile("s_nop 4\n\t"
+                 "global_load_lds_dwordx4 %0, %1"
+                 :
+                 : "v"(byte_offset), "s"(base), "{m0}"(lds_base)
+                 : "memory");
+}
+__device__ __forceinline__ void load4(const void *base, uint32_t byte_offset, uint32_t lds_base) {
+    asm volatile("s_nop 4\n\t"
+                 "global_load_lds_dword %0, %1"
+                 :
+                 : "v"(byte_offset), "s"(base), "{m0}"(lds_base)
+                 : "memory");
+}
+// an address that is the same in every lane, where the compiler does not see that it is
+template <typename P> __device__ __forceinline__ const P *same_in_lanes(const P *p) {
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    return reinterpret_cast<const P *>((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 |
+                                       (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
+
+// EDGE: some tile of the launch has rows beyond an operand, whose place its last row takes.
+template <typename O, int WM, int WN, int MT, int NT, bool EDGE>
+__global__ __launch_bounds__(WM * WN * 64, 2) void gemm_f8_dma_kernel(F8Args a, uint32_t tiles_m, uint32_t tiles_n) {
+    using T = DmaTile<O, WM, WN, MT, NT>;
+    using namespace lds_dma;
+    __shared__ __align__(1024) uint8_t lds[2 * T::HALF];
+    uint32_t tm, tn;
+    tile_place(blockIdx.x, tiles_m * tiles_n, tiles_m, tiles_n, tm, tn);
+    tm = __builtin_amdgcn_readfirstlane(tm); // (the division left them in vector registers)
+    tn = __builtin_amdgcn_readfirstlane(tn);
+    const uint32_t m0 = tm * T::TM, n0 = tn * T::TN;
+    const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t wm = (wave % WM) * (MT * 16), wn = (wave / WM) * (NT * 16);
+    const uint32_t r16 = lane % 16, g = lane / 16;
+    const uint32_t whole = a.K / KB;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
+
+    // Loads: instruction q of this wavefront fills the 1 KiB piece q * waves + wave of an operand (eight rows); lane l of it the chunk
+    // l % 8 of row l / 8, which is the row's chunk (l % 8) ^ (row % 8).
+    constexpr uint32_t WAVES = WM * WN, QA = T::A_BYTES / 1024 / WAVES, QB = T::B_BYTES / 1024 / WAVES;
+    const uint32_t lda = (uint32_t)a.lda, ldb = (uint32_t)a.ldb;
+    const uint32_t lrow = wave * 8 + lane / 8, lchunk = ((lane % 8) ^ (lane / 8)) * 16;
+    const uint32_t last_a = a.M - 1 - m0, last_b = a.N - 1 - n0;
+    auto row_a = [&](uint32_t q) {
+        const uint32_t r = q * WAVES * 8 + lrow;
+        return (EDGE && r > last_a ? last_a : r) * lda;
+    };
+    auto row_b = [&](uint32_t q) {
+        const uint32_t r = q * WAVES * 8 + lrow;
+        return (EDGE && r > last_b ? last_b : r) * ldb;
+    };
+    const uint32_t off_a = row_a(0) + lchunk, off_b = row_b(0) + lchunk;
+    // Scales: wavefront w brings 64 of A's, rows 64 w ..., in the order in which a lane will want them: place p of 16 MT rows holds row
+    // (p % MT) * 16 + p / MT; the wavefronts that are left bring B's, one per 128 columns (all the same ones: a branch here would
+    // end the loop's basic block, and what is behind it would be kept waiting)
+    const bool for_a = wave * 64 < T::TM;
+    uint32_t off_s;
+    {
+        const uint32_t p = wave * 64 + lane, rows = MT * 16, base = p / rows * rows, in = p - base;
+        const uint32_t r = base + (in % MT) * 16 + in / MT;
+        off_s = for_a ? (r < last_a ? r : last_a) * (uint32_t)a.sap * 4 : (lane < T::NB && lane * KB <= last_b ? lane : 0) * (uint32_t)a.sbp * 4;
+    }
+    const uint8_t *base_a = a.A + (uint64_t)m0 * a.lda, *base_b = a.B + (uint64_t)n0 * a.ldb;
+    const float *base_s = same_in_lanes(for_a ? a.sa + (uint64_t)m0 * a.sap : a.sb + (uint64_t)(n0 / KB) * a.sbp);
+
+    auto request_scales = [&](uint32_t kb, uint32_t half) {
+        load4(same_in_lanes(base_s + kb), off_s, lds0 + half + T::A_BYTES + T::B_BYTES + wave * 256);
+    };
+    auto request = [&](uint32_t kb, uint32_t half) {
+        const uint8_t *ka = base_a + (uint64_t)kb * KB, *kbp = base_b + (uint64_t)kb * KB;
+        const uint32_t to = lds0 + half + wave * 1024;
+#pragma unroll
+        for (uint32_t q = 0; q < QA; ++q) {
+            if (EDGE && q) load16(ka, row_a(q) + lchunk, to + q * WAVES * 1024);
+            else load16(ka + (uint64_t)(q * WAVES * 8) * lda, off_a, to + q * WAVES * 1024);
+        }
+#pragma unroll
+        for (uint32_t q = 0; q < QB; ++q) {
+            if (EDGE && q) load16(kbp, row_b(q) + lchunk, to + T::A_BYTES + q * WAVES * 1024);
+            else load16(kbp + (uint64_t)(q * WAVES * 8) * ldb, off_b, to + T::A_BYTES + q * WAVES * 1024);
+        }
+        request_scales(kb, half);
+    };
+    // the shorter last block: through registers, zeros behind K (once per tile: rolled, and its addresses formed here and not before
+    // the loop over k, which has no registers left for them)
+    auto stage_short = [&](uint32_t kb, uint32_t half) {
+        uint32_t r0 = lrow;
+        asm volatile("" : "+v"(r0));
+#pragma unroll 1
+        for (uint32_t q = 0; q < QA + QB; ++q) {
+            const bool is_a = q < QA;
+            const uint32_t r = (is_a ? q : q - QA) * WAVES * 8 + r0, last = is_a ? last_a : last_b;
+            const uint8_t *row = (is_a ? base_a : base_b) + (uint64_t)(r < last ? r : last) * (is_a ? lda : ldb);
+            *reinterpret_cast<i32x4 *>(lds + half + (is_a ? 0 : T::A_BYTES) + ((is_a ? q : q - QA) * WAVES + wave) * 1024 + lane * 16) =
+                load_chunk<true>(row, kb * KB + lchunk, a.K);
+        }
+        request_scales(kb, half);
+    };
+    const uint32_t at_a = (wm + r16) * KB, at_b = T::A_BYTES + (wn + r16) * KB; // (rows 16 apart have the same swizzle)
+    const uint32_t lo = (g ^ (r16 & 7)) << 4, hi = lo ^ 64;
+    auto operand = [&](uint32_t at) {
+        return __builtin_shufflevector(*reinterpret_cast<const i32x4 *>(lds + at + lo), *reinterpret_cast<const i32x4 *>(lds + at + hi), 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+
+    f32x4 acc[MT][NT] = {};
+    i32x8 fb[NT], fa[2];
+    float s[MT], s_b;
+    auto read_scales = [&](uint32_t half) {
+        const float *p = reinterpret_cast<const float *>(lds + half + T::A_BYTES + T::B_BYTES);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) s[i] = p[wm + r16 * MT + i];
+        s_b = p[T::TM + wn / KB];
+    };
+    auto first_operands = [&](uint32_t half) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) fb[j] = operand(half + at_b + 16 * j * KB);
+        fa[0] = operand(half + at_a);
+        read_scales(half);
+    };
+    // the products of the block in `half`; MORE: on the way the next one's first operands, and the request of block `ahead`
+    auto block = [&]<bool MORE>(std::integral_constant<bool, MORE>, uint32_t half, uint32_t ahead) {
+        decltype(operand_of<O>(i32x8{})) wb[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) wb[j] = operand_of<O>(fb[j]);
+        // one step: a product is started, the one started LAG steps before is scaled and added.  The order is held as written: a
+        // free schedule lets so many results live at once that registers spill.
+        constexpr int LAG = 3;
+        f32x4 p[LAG + 1];
+        decltype(operand_of<O>(i32x8{})) wa;
+#pragma unroll
+        for (int t = 0; t < MT * NT + LAG; ++t) {
+            const int i = t / NT, j = t % NT;
+            if (t < MT * NT) {
+                if (j == 0) {
+                    wa = operand_of<O>(fa[i & 1]);
+                    if (i + 1 < MT) {
+                        fa[(i + 1) & 1] = operand(half + at_a + 16 * (i + 1) * KB);
+                    } else if (MORE) {
+                        wait_lgkm0(); // this wavefront has read the block,
+                        wait_vm<0>(); // and its share of the next one is there
+                        __builtin_amdgcn_s_barrier();
+                        asm volatile("" ::: "memory");
+                        request(ahead, half);
+                        fa[(i + 1) & 1] = operand(T::HALF - half + at_a);
+                    }
+                }
+                p[t % (LAG + 1)] = mfma_block(wb[j], wa, f32x4{0.f, 0.f, 0.f, 0.f});
+                if (i + 1 == MT && MORE) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    fb[j] = operand(T::HALF - half + at_b + 16 * j * KB);
+                }
+            }
+            if (t >= LAG) {
+                const int u = t - LAG, k = u / NT;
+                const float f = s[k] * s_b;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[k][u % NT][e] = __builtin_fmaf(p[u % (LAG + 1)][e], f, acc[k][u % NT][e]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (MORE) read_scales(T::HALF - half);
+    };
+
+    uint32_t half = 0;
+    if (whole) {
+        request(0, 0);
+        request(whole > 1 ? 1 : 0, T::HALF);
+        wait_vm<0>();
+        __syncthreads();
+        first_operands(0);
+        // (the last request repeats a block into the half that nobody reads any more)
+        for (uint32_t kb = 0; kb + 1 < whole; ++kb) {
+            block(std::true_type{}, half, kb + 2 < whole ? kb + 2 : kb + 1);
+            half = T::HALF - half;
+        }
+    }
+#pragma unroll 1
+    for (uint32_t kb = whole ? whole - 1 : 0; kb < a.kblocks; ++kb) {
+        if (kb == whole) {
+            wait_vm<0>();
+            __syncthreads();
+            half = T::HALF - half;
+            stage_short(kb, half);
+            wait_vm<0>();
+            __syncthreads();
+            first_operands(half);
+        }
+        block(std::false_type{}, half, 0);
+    }
+    wait_vm<0>();
+
+    if (a.kind == WK_ACT_NONE) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) store_row4<O, false>(a, m0 + wm + 16 * i + r16, n0 + wn + 16 * j + 4 * g, acc[i][j]);
+        return;
+    }
+    // with an activation: through LDS, each lane its own, so that its code is there once
+    constexpr int PASS = 2 * T::HALF / (16 * T::THREADS) < MT * NT ? MT * NT / 2 : MT * NT;
+    static_assert(PASS * 16 * T::THREADS <= 2 * T::HALF);
+    __syncthreads();
+    f32x4 *own = reinterpret_cast<f32x4 *>(lds) + threadIdx.x;
+#pragma unroll
+    for (int first = 0; first < MT * NT; first += PASS) {
+#pragma unroll
+        for (int q = 0; q < PASS; ++q) own[q * T::THREADS] = acc[(first + q) / NT][(first + q) % NT];
+#pragma unroll 1
+        for (int q = 0; q < PASS; ++q)
+            store_row4<O, true>(a, m0 + wm + 16 * ((first + q) / NT) + r16, n0 + wn + 16 * ((first + q) % NT) + 4 * g, own[q * T::THREADS]);
+    }
+}
+
+template <typename O, int WM, int WN, int MT, int NT> int gemm_f8_dma_launch(hipStream_t st, const F8Args &a) {
+    using T = DmaTile<O, WM, WN, MT, NT>;
+    const uint64_t tiles_m = (a.M + T::TM - 1) / T::TM, tiles_n = (a.N + T::TN - 1) / T::TN;
+    if (tiles_m * tiles_n > 0x7fffffffull) return WK_E_INVALID_VALUE;
+    const dim3 grid((unsigned)(tiles_m * tiles_n)), block(T::THREADS);
+    if (a.M % T::TM || a.N % T::TN)
+        hipLaunchKernelGGL((gemm_f8_dma_kernel<O, WM, WN, MT, NT, true>), grid, block, 0, st, a, (uint32_t)tiles_m, (uint32_t)tiles_n);
+    else
+        hipLaunchKernelGGL((gemm_f8_dma_kernel<O, WM, WN, MT, NT, false>), grid, block, 0, st, a, (uint32_t)tiles_m, (uint32_t)tiles_n);
+    return launch_status();
 }
 
 // Few rows: 16 MT rows of A against 16 NT rows of B, which is streamed once from memory straight into the lanes' operand
@@ -274,14 +530,23 @@ template <bool ALIGNED, typename O> int gemm_f8_rows_launch(hipStream_t st, cons
     if (a.M <= 16)
         hipLaunchKernelGGL((gemm_f8_rows_kernel<ALIGNED, O, 1, 1, 4>), dim3((a.N + 15) / 16), block, 0, st, a);
     else if (a.M <= 32)
-        hipLaunchKernelGGL((gemm_f8_rows_kernel<ALIGNED, O, 2, 1, 4>), dim3((a.N + 15) / 16), block, 0, st, a);
+        hipLaunchKernelGGL((gemm_f8_rows_kernel<ALIGNED, O, 2, 2, 2>), dim3((a.N + 31) / 32), block, 0, st, a);
     else
-        hipLaunchKernelGGL((gemm_f8_rows_kernel<ALIGNED, O, 4, 1, 2>), dim3((a.N + 15) / 16, (a.M + 63) / 64), block, 0, st, a);
+        hipLaunchKernelGGL((gemm_f8_rows_kernel<ALIGNED, O, 4, 2, 2>), dim3((a.N + 31) / 32, (a.M + 63) / 64), block, 0, st, a);
     return launch_status();
 }
 
 template <typename O> int gemm_f8_launch(wk_stream *s, const F8Args &a, bool aligned) {
     if (a.M <= 64) return aligned ? gemm_f8_rows_launch<true, O>(s->stream, a) : gemm_f8_rows_launch<false, O>(s->stream, a);
+    // lane offsets within a tile are 32 bits
+    if (aligned && a.lda < (1u << 23) && a.ldb < (1u << 23) && a.sap < (1u << 21) && a.sbp < (1u << 21)) {
+        if constexpr (std::is_same_v<O, float>) {
+            return gemm_f8_dma_launch<O, 2, 2, 4, 4>(s->stream, a);
+        } else {
+            if ((uint64_t)a.M * a.N >= (uint64_t)256 * 256 * 200) return gemm_f8_dma_launch<O, 2, 4, 8, 4>(s->stream, a);
+            return gemm_f8_dma_launch<O, 2, 2, 4, 4>(s->stream, a);
+        }
+    }
     const uint64_t tiles = (uint64_t)((a.M + 127) / 128) * ((a.N + 127) / 128);
     if (tiles > 0x7fffffffull) return WK_E_INVALID_VALUE;
     if (aligned)
