@@ -66,10 +66,32 @@ __device__ __forceinline__ f32x4 mfma_block(const Wide &rows, const Wide &cols, 
     for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(rows.v[i], cols.v[i], acc, 0, 0, 0);
     return acc;
 }
+// one block's products of several operands of B with one of A, started in turns
+template <int STEP> __device__ __forceinline__ void start(const i32x8 *rows, i32x8 cols, f32x4 *p) {
+#pragma unroll
+    for (int q = 0; q < STEP; ++q) p[q] = mfma_block(rows[q], cols, f32x4{0.f, 0.f, 0.f, 0.f});
+}
+template <int STEP> __device__ __forceinline__ void start(const Wide *rows, const Wide &cols, f32x4 *p) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int q = 0; q < STEP; ++q)
+            p[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rows[q].v[i], cols.v[i], i ? p[q] : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+}
 // what a lane's codes become before they are multiplied, by the result's type
 template <typename O> __device__ __forceinline__ auto operand_of(i32x8 c) {
     if constexpr (std::is_same_v<O, float>) return widen_codes(c);
     else return c;
+}
+
+// the first n < 16 bytes of a chunk, zeros behind them
+__device__ __forceinline__ i32x4 first_bytes(i32x4 v, uint32_t n) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const int bytes = (int)n - 4 * w; // of this word that stay
+        v[w] = bytes >= 4 ? v[w] : bytes <= 0 ? 0 : v[w] & (int)((1u << (8 * bytes)) - 1u);
+    }
+    return v;
 }
 
 // 16 bytes of a row from byte k on; bytes at and beyond K are zero
@@ -79,13 +101,7 @@ template <bool ALIGNED> __device__ __forceinline__ i32x4 load_chunk(const uint8_
     const uint32_t left = K - k;
     if (ALIGNED) {
         v = *reinterpret_cast<const i32x4 *>(row + k);
-        if (left < 16) {
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const int bytes = (int)left - 4 * w; // of this word that exist
-                v[w] = bytes >= 4 ? v[w] : bytes <= 0 ? 0 : v[w] & (int)((1u << (8 * bytes)) - 1u);
-            }
-        }
+        if (left < 16) v = first_bytes(v, left);
     } else {
 #pragma unroll
         for (int e = 0; e < 16; ++e)
@@ -190,17 +206,16 @@ template <bool ALIGNED, typename O> __global__ __launch_bounds__(256) void gemm_
 }
 
 // The kernel for aligned operands.  WM x WN wavefronts with 16 MT x 16 NT of C each; k-blocks go from memory straight into
-// LDS, two of them at a time in the two halves of it (rows and chunks as above, the swizzle on the source's side), the scales
-// with them.
+// LDS, which holds STAGES of them (rows and chunks as above, the swizzle on the source's side), the scales with them.
 //
 // Per block a wavefront reads its NT operands of B once and its MT operands of A one ahead of use.  When the last of them
-// is in registers the wavefronts meet: the block is read, the next one has landed (it was asked for a whole block ago), the one after
-// that is asked for, and the next block's first operands are read while the last row of products still runs.
-template <typename O, int WM, int WN, int MT, int NT> struct DmaTile {
+// is in registers the wavefronts meet: the block is read, the next one has landed (it was asked for STAGES - 1 blocks ago), its stage is
+// asked to be filled again, and the next block's first operands are read while the last row of products still runs.
+template <typename O, int WM, int WN, int MT, int NT, int STAGES> struct DmaTile {
     static constexpr uint32_t TM = WM * MT * 16, TN = WN * NT * 16, THREADS = WM * WN * 64;
     static constexpr uint32_t NB = TN > KB ? TN / KB : 1; // rows of B's scales
     static constexpr uint32_t A_BYTES = TM * KB, B_BYTES = TN * KB, SCALE_BYTES = WM * WN * 256; // (64 scales per wavefront)
-    static constexpr uint32_t HALF = A_BYTES + B_BYTES + SCALE_BYTES;
+    static constexpr uint32_t STAGE = A_BYTES + B_BYTES + SCALE_BYTES, LDS = STAGES * STAGE;
     static_assert(TM % 64 == 0 && TM / 64 < WM * WN && A_BYTES % (16 * THREADS) == 0 && B_BYTES % (16 * THREADS) == 0 && NB <= 64);
 };
 
@@ -240,11 +255,11 @@ template <typename P> __device__ __forceinline__ const P *same_in_lanes(const P 
 }
 
 // EDGE: some tile of the launch has rows beyond an operand, whose place its last row takes.
-template <typename O, int WM, int WN, int MT, int NT, bool EDGE>
+template <typename O, int WM, int WN, int MT, int NT, int STAGES, bool EDGE>
 __global__ __launch_bounds__(WM * WN * 64, 2) void gemm_f8_dma_kernel(F8Args a, uint32_t tiles_m, uint32_t tiles_n) {
-    using T = DmaTile<O, WM, WN, MT, NT>;
+    using T = DmaTile<O, WM, WN, MT, NT, STAGES>;
     using namespace lds_dma;
-    __shared__ __align__(1024) uint8_t lds[2 * T::HALF];
+    __shared__ __align__(1024) uint8_t lds[T::LDS];
     uint32_t tm, tn;
     tile_place(blockIdx.x, tiles_m * tiles_n, tiles_m, tiles_n, tm, tn);
     tm = __builtin_amdgcn_readfirstlane(tm); // (the division left them in vector registers)
@@ -271,6 +286,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void gemm_f8_dma_kernel(F8Args a, 
         return (EDGE && r > last_b ? last_b : r) * ldb;
     };
     const uint32_t off_a = row_a(0) + lchunk, off_b = row_b(0) + lchunk;
+    // In the shorter last block the chunks behind K repeat the last one that has some of it (and are put to zero later).
+    const uint32_t rest = a.K % KB, beyond = rest && lchunk > (rest - 1) / 16 * 16 ? lchunk - (rest - 1) / 16 * 16 : 0;
     // Scales: wavefront w brings 64 of A's, rows 64 w ..., in the order in which a lane will want them: place p of 16 MT rows holds row
     // (p % MT) * 16 + p / MT; the wavefronts that are left bring B's, one per 128 columns (all the same ones: a branch here would
     // end the loop's basic block, and what is behind it would be kept waiting)
@@ -284,38 +301,38 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void gemm_f8_dma_kernel(F8Args a, 
     const uint8_t *base_a = a.A + (uint64_t)m0 * a.lda, *base_b = a.B + (uint64_t)n0 * a.ldb;
     const float *base_s = same_in_lanes(for_a ? a.sa + (uint64_t)m0 * a.sap : a.sb + (uint64_t)(n0 / KB) * a.sbp);
 
-    auto request_scales = [&](uint32_t kb, uint32_t half) {
-        load4(same_in_lanes(base_s + kb), off_s, lds0 + half + T::A_BYTES + T::B_BYTES + wave * 256);
+    auto request_scales = [&](uint32_t kb, uint32_t at) {
+        load4(same_in_lanes(base_s + kb), off_s, lds0 + at + T::A_BYTES + T::B_BYTES + wave * 256);
     };
-    auto request = [&](uint32_t kb, uint32_t half) {
-        const uint8_t *ka = base_a + (uint64_t)kb * KB, *kbp = base_b + (uint64_t)kb * KB;
-        const uint32_t to = lds0 + half + wave * 1024;
-#pragma unroll
-        for (uint32_t q = 0; q < QA; ++q) {
-            if (EDGE && q) load16(ka, row_a(q) + lchunk, to + q * WAVES * 1024);
-            else load16(ka + (uint64_t)(q * WAVES * 8) * lda, off_a, to + q * WAVES * 1024);
+    constexpr uint32_t PER = QA + QB + 1; // loads of a wavefront per block
+    auto request_one = [&](uint32_t kb, uint32_t at, uint32_t n) {
+        const uint32_t to = lds0 + at + wave * 1024, back = kb < whole ? 0 : beyond;
+        if (n < QA) {
+            const uint8_t *ka = base_a + (uint64_t)kb * KB;
+            if (EDGE && n) load16(ka, row_a(n) + lchunk - back, to + n * WAVES * 1024);
+            else load16(ka + (uint64_t)(n * WAVES * 8) * lda, off_a - back, to + n * WAVES * 1024);
+        } else if (n < QA + QB) {
+            const uint32_t q = n - QA;
+            const uint8_t *kbp = base_b + (uint64_t)kb * KB;
+            if (EDGE && q) load16(kbp, row_b(q) + lchunk - back, to + T::A_BYTES + q * WAVES * 1024);
+            else load16(kbp + (uint64_t)(q * WAVES * 8) * ldb, off_b - back, to + T::A_BYTES + q * WAVES * 1024);
+        } else {
+            request_scales(kb, at);
         }
-#pragma unroll
-        for (uint32_t q = 0; q < QB; ++q) {
-            if (EDGE && q) load16(kbp, row_b(q) + lchunk, to + T::A_BYTES + q * WAVES * 1024);
-            else load16(kbp + (uint64_t)(q * WAVES * 8) * ldb, off_b, to + T::A_BYTES + q * WAVES * 1024);
-        }
-        request_scales(kb, half);
     };
-    // the shorter last block: through registers, zeros behind K (once per tile: rolled, and its addresses formed here and not before
-    // the loop over k, which has no registers left for them)
-    auto stage_short = [&](uint32_t kb, uint32_t half) {
-        uint32_t r0 = lrow;
-        asm volatile("" : "+v"(r0));
+    auto request = [&](uint32_t kb, uint32_t at) {
+#pragma unroll
+        for (uint32_t n = 0; n < PER; ++n) request_one(kb, at, n);
+    };
+    // zeros behind K in the shorter last block
+    auto cut_short = [&](uint32_t at) {
 #pragma unroll 1
-        for (uint32_t q = 0; q < QA + QB; ++q) {
-            const bool is_a = q < QA;
-            const uint32_t r = (is_a ? q : q - QA) * WAVES * 8 + r0, last = is_a ? last_a : last_b;
-            const uint8_t *row = (is_a ? base_a : base_b) + (uint64_t)(r < last ? r : last) * (is_a ? lda : ldb);
-            *reinterpret_cast<i32x4 *>(lds + half + (is_a ? 0 : T::A_BYTES) + ((is_a ? q : q - QA) * WAVES + wave) * 1024 + lane * 16) =
-                load_chunk<true>(row, kb * KB + lchunk, a.K);
+        for (uint32_t c = threadIdx.x; c < (T::TM + T::TN) * 8; c += T::THREADS) {
+            i32x4 *chunk = reinterpret_cast<i32x4 *>(lds + at) + c;
+            const uint32_t k = ((c % 8) ^ (c / 8 % 8)) * 16;
+            if (k + 16 <= rest) continue;
+            *chunk = k >= rest ? i32x4{0, 0, 0, 0} : first_bytes(*chunk, rest - k);
         }
-        request_scales(kb, half);
     };
     const uint32_t at_a = (wm + r16) * KB, at_b = T::A_BYTES + (wn + r16) * KB; // (rows 16 apart have the same swizzle)
     const uint32_t lo = (g ^ (r16 & 7)) << 4, hi = lo ^ 64;
@@ -326,87 +343,97 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void gemm_f8_dma_kernel(F8Args a, 
     f32x4 acc[MT][NT] = {};
     i32x8 fb[NT], fa[2];
     float s[MT], s_b;
-    auto read_scales = [&](uint32_t half) {
-        const float *p = reinterpret_cast<const float *>(lds + half + T::A_BYTES + T::B_BYTES);
+    auto read_scales = [&](uint32_t at) {
+        const float *p = reinterpret_cast<const float *>(lds + at + T::A_BYTES + T::B_BYTES);
 #pragma unroll
         for (int i = 0; i < MT; ++i) s[i] = p[wm + r16 * MT + i];
         s_b = p[T::TM + wn / KB];
     };
-    auto first_operands = [&](uint32_t half) {
+    auto first_operands = [&](uint32_t at) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) fb[j] = operand(half + at_b + 16 * j * KB);
-        fa[0] = operand(half + at_a);
-        read_scales(half);
+        for (int j = 0; j < NT; ++j) fb[j] = operand(at + at_b + 16 * j * KB);
+        fa[0] = operand(at + at_a);
+        read_scales(at);
     };
-    // the products of the block in `half`; MORE: on the way the next one's first operands, and the request of block `ahead`
-    auto block = [&]<bool MORE>(std::integral_constant<bool, MORE>, uint32_t half, uint32_t ahead) {
+    // the products of the block at `at`; MORE: on the way the first operands of the next one, at `next`, and the request of block `ahead`
+    auto block = [&]<bool MORE>(std::integral_constant<bool, MORE>, uint32_t at, uint32_t next, uint32_t ahead) {
         decltype(operand_of<O>(i32x8{})) wb[NT];
 #pragma unroll
         for (int j = 0; j < NT; ++j) wb[j] = operand_of<O>(fb[j]);
-        // one step: a product is started, the one started LAG steps before is scaled and added.  The order is held as written: a
-        // free schedule lets so many results live at once that registers spill.
-        constexpr int LAG = 3;
-        f32x4 p[LAG + 1];
+        // One step: STEP products of a row are started, those of the step LAG before are scaled and added.  f32: a whole row, whose
+        // four instructions each take turns (each waits for the one before it in its sum).  The order is held as written: a free
+        // schedule lets so many results live at once that registers spill.
+        constexpr bool WIDE = std::is_same_v<O, float>;
+        constexpr int STEP = WIDE ? NT : 1, LAG = WIDE ? 1 : 3, STEPS = MT * NT / STEP;
+        f32x4 p[LAG + 1][STEP];
         decltype(operand_of<O>(i32x8{})) wa;
 #pragma unroll
-        for (int t = 0; t < MT * NT + LAG; ++t) {
-            const int i = t / NT, j = t % NT;
-            if (t < MT * NT) {
+        for (int t = 0; t < STEPS + LAG; ++t) {
+            const int i = t * STEP / NT, j = t * STEP % NT;
+            if (t < STEPS) {
                 if (j == 0) {
                     wa = operand_of<O>(fa[i & 1]);
                     if (i + 1 < MT) {
-                        fa[(i + 1) & 1] = operand(half + at_a + 16 * (i + 1) * KB);
+                        fa[(i + 1) & 1] = operand(at + at_a + 16 * (i + 1) * KB);
                     } else if (MORE) {
                         wait_lgkm0(); // this wavefront has read the block,
-                        wait_vm<0>(); // and its share of the next one is there
+                        wait_vm<(STAGES - 2) * PER>(); // and its share of the next one is there
                         __builtin_amdgcn_s_barrier();
                         asm volatile("" ::: "memory");
-                        request(ahead, half);
-                        fa[(i + 1) & 1] = operand(T::HALF - half + at_a);
                     }
                 }
-                p[t % (LAG + 1)] = mfma_block(wb[j], wa, f32x4{0.f, 0.f, 0.f, 0.f});
+                start<STEP>(&wb[j], wa, p[t % (LAG + 1)]);
                 if (i + 1 == MT && MORE) {
+                    // the next block's operands, and requests to refill this one's stage, under the running products
                     __builtin_amdgcn_sched_barrier(0);
-                    fb[j] = operand(T::HALF - half + at_b + 16 * j * KB);
+                    if (j == 0) fa[(i + 1) & 1] = operand(next + at_a);
+#pragma unroll
+                    for (int q = j; q < j + STEP; ++q) fb[q] = operand(next + at_b + 16 * q * KB);
+#pragma unroll
+                    for (uint32_t n = j * PER / NT; n < (j + STEP) * PER / NT; ++n) request_one(ahead, at, n);
                 }
             }
             if (t >= LAG) {
-                const int u = t - LAG, k = u / NT;
+                const int u = t - LAG, k = u * STEP / NT;
                 const float f = s[k] * s_b;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[k][u % NT][e] = __builtin_fmaf(p[u % (LAG + 1)][e], f, acc[k][u % NT][e]);
+                for (int q = 0; q < STEP; ++q)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        acc[k][u * STEP % NT + q][e] = __builtin_fmaf(p[u % (LAG + 1)][q][e], f, acc[k][u * STEP % NT + q][e]);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
-        if (MORE) read_scales(T::HALF - half);
+        if (MORE) read_scales(next);
     };
 
-    uint32_t half = 0;
+    uint32_t at = 0;
+    auto after = [](uint32_t stage) { return stage + T::STAGE == T::LDS ? 0 : stage + T::STAGE; };
+    // (requests beyond the last block repeat it, into stages that nobody reads any more: the counts stay the same)
+    const uint32_t last_block = a.kblocks - 1;
+#pragma unroll
+    for (uint32_t q = 0; q < STAGES; ++q) request(q < last_block ? q : last_block, q * T::STAGE);
     if (whole) {
-        request(0, 0);
-        request(whole > 1 ? 1 : 0, T::HALF);
-        wait_vm<0>();
+        wait_vm<(STAGES - 1) * PER>();
         __syncthreads();
         first_operands(0);
-        // (the last request repeats a block into the half that nobody reads any more)
         for (uint32_t kb = 0; kb + 1 < whole; ++kb) {
-            block(std::true_type{}, half, kb + 2 < whole ? kb + 2 : kb + 1);
-            half = T::HALF - half;
+            const uint32_t next = after(at);
+            block(std::true_type{}, at, next, kb + STAGES < last_block ? kb + STAGES : last_block);
+            at = next;
         }
     }
 #pragma unroll 1
-    for (uint32_t kb = whole ? whole - 1 : 0; kb < a.kblocks; ++kb) {
-        if (kb == whole) {
+    for (uint32_t kb = whole ? whole - 1 : 0; kb <= last_block; ++kb) {
+        if (kb == whole) { // the shorter one
+            if (whole) at = after(at);
             wait_vm<0>();
             __syncthreads();
-            half = T::HALF - half;
-            stage_short(kb, half);
-            wait_vm<0>();
+            cut_short(at);
             __syncthreads();
-            first_operands(half);
+            first_operands(at);
         }
-        block(std::false_type{}, half, 0);
+        block(std::false_type{}, at, 0, 0);
     }
     wait_vm<0>();
 
@@ -418,8 +445,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void gemm_f8_dma_kernel(F8Args a, 
         return;
     }
     // with an activation: through LDS, each lane its own, so that its code is there once
-    constexpr int PASS = 2 * T::HALF / (16 * T::THREADS) < MT * NT ? MT * NT / 2 : MT * NT;
-    static_assert(PASS * 16 * T::THREADS <= 2 * T::HALF);
+    constexpr int PASS = T::LDS / (16 * T::THREADS) < MT * NT ? MT * NT / 2 : MT * NT;
+    static_assert(PASS * 16 * T::THREADS <= T::LDS);
     __syncthreads();
     f32x4 *own = reinterpret_cast<f32x4 *>(lds) + threadIdx.x;
 #pragma unroll
@@ -432,23 +459,24 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void gemm_f8_dma_kernel(F8Args a, 
     }
 }
 
-template <typename O, int WM, int WN, int MT, int NT> int gemm_f8_dma_launch(hipStream_t st, const F8Args &a) {
-    using T = DmaTile<O, WM, WN, MT, NT>;
+template <typename O, int WM, int WN, int MT, int NT, int STAGES> int gemm_f8_dma_launch(hipStream_t st, const F8Args &a) {
+    using T = DmaTile<O, WM, WN, MT, NT, STAGES>;
     const uint64_t tiles_m = (a.M + T::TM - 1) / T::TM, tiles_n = (a.N + T::TN - 1) / T::TN;
     if (tiles_m * tiles_n > 0x7fffffffull) return WK_E_INVALID_VALUE;
     const dim3 grid((unsigned)(tiles_m * tiles_n)), block(T::THREADS);
     if (a.M % T::TM || a.N % T::TN)
-        hipLaunchKernelGGL((gemm_f8_dma_kernel<O, WM, WN, MT, NT, true>), grid, block, 0, st, a, (uint32_t)tiles_m, (uint32_t)tiles_n);
+        hipLaunchKernelGGL((gemm_f8_dma_kernel<O, WM, WN, MT, NT, STAGES, true>), grid, block, 0, st, a, (uint32_t)tiles_m, (uint32_t)tiles_n);
     else
-        hipLaunchKernelGGL((gemm_f8_dma_kernel<O, WM, WN, MT, NT, false>), grid, block, 0, st, a, (uint32_t)tiles_m, (uint32_t)tiles_n);
+        hipLaunchKernelGGL((gemm_f8_dma_kernel<O, WM, WN, MT, NT, STAGES, false>), grid, block, 0, st, a, (uint32_t)tiles_m, (uint32_t)tiles_n);
     return launch_status();
 }
 
 // Few rows: 16 MT rows of A against 16 NT rows of B, which is streamed once from memory straight into the lanes' operand
 // registers (both operands assign k to lanes alike, and a sum does not care which k that is).  The eight wavefronts of a
 // work-group take every eighth block of k, DEEP of them in flight each, and their sums meet in LDS in wavefront order.
-template <bool ALIGNED, typename O, int MT, int NT, int DEEP> __global__ __launch_bounds__(512) void gemm_f8_rows_kernel(F8Args a) {
-    constexpr uint32_t WAVES = 8;
+// Work-groups start their walk along k at different places: rows a power of two apart lie in the same memory channel, and all
+// work-groups would go through the channels in step.
+template <bool ALIGNED, typename O, int MT, int NT, int DEEP, uint32_t WAVES = 8> __global__ __launch_bounds__(WAVES * 64) void gemm_f8_rows_kernel(F8Args a) {
     __shared__ f32x4 part[WAVES][MT * NT][64];
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, r16 = lane % 16, g = lane / 16;
     const uint32_t n0 = blockIdx.x * (16 * NT), m0 = blockIdx.y * (16 * MT);
@@ -501,15 +529,25 @@ template <bool ALIGNED, typename O, int MT, int NT, int DEEP> __global__ __launc
             }
         }
     };
-    uint32_t kb = wave;
-    for (; kb + (DEEP - 1) * WAVES < whole; kb += DEEP * WAVES) {
+    const uint32_t mine = whole > wave ? (whole - wave - 1) / WAVES + 1 : 0; // whole blocks of this wavefront
+    uint32_t turn = mine ? blockIdx.x % mine : 0, done = 0;
+    auto next_block = [&]() {
+        const uint32_t kb = wave + turn * WAVES;
+        turn = turn + 1 == mine ? 0 : turn + 1;
+        return kb;
+    };
+    for (; done + DEEP <= mine; done += DEEP) {
 #pragma unroll
-        for (int d = 0; d < DEEP; ++d) fetch(d, kb + d * WAVES, true);
+        for (int d = 0; d < DEEP; ++d) fetch(d, next_block(), true);
 #pragma unroll
         for (int d = 0; d < DEEP; ++d) multiply(d);
     }
-    for (; kb < a.kblocks; kb += WAVES) {
-        fetch(0, kb, kb < whole);
+    for (; done < mine; ++done) {
+        fetch(0, next_block(), true);
+        multiply(0);
+    }
+    if (whole < a.kblocks && whole % WAVES == wave) { // the shorter last one
+        fetch(0, whole, false);
         multiply(0);
     }
 #pragma unroll
@@ -525,34 +563,75 @@ template <bool ALIGNED, typename O, int MT, int NT, int DEEP> __global__ __launc
     }
 }
 
-template <bool ALIGNED, typename O> int gemm_f8_rows_launch(hipStream_t st, const F8Args &a) {
-    const dim3 block(512);
-    if (a.M <= 16)
-        hipLaunchKernelGGL((gemm_f8_rows_kernel<ALIGNED, O, 1, 1, 4>), dim3((a.N + 15) / 16), block, 0, st, a);
-    else if (a.M <= 32)
-        hipLaunchKernelGGL((gemm_f8_rows_kernel<ALIGNED, O, 2, 2, 2>), dim3((a.N + 31) / 32), block, 0, st, a);
-    else
-        hipLaunchKernelGGL((gemm_f8_rows_kernel<ALIGNED, O, 4, 2, 2>), dim3((a.N + 31) / 32, (a.M + 63) / 64), block, 0, st, a);
+template <bool ALIGNED, typename O, int MT, int NT, int DEEP, uint32_t WAVES = 8> int gemm_f8_rows_launch(hipStream_t st, const F8Args &a) {
+    hipLaunchKernelGGL((gemm_f8_rows_kernel<ALIGNED, O, MT, NT, DEEP, WAVES>), dim3((a.N + 16 * NT - 1) / (16 * NT), (a.M + 16 * MT - 1) / (16 * MT)),
+                       dim3(WAVES * 64), 0, st, a);
     return launch_status();
 }
 
+// Up to 64 rows.  Measured (f32 results, us; N = K = 8192 unless said): 8 rows 16 columns at a time 19.5, 32 columns and sixteen
+// wavefronts 17.7, but 9.8 against 13.0 at N = 2048, where those leave three quarters of the units without work; 32 rows 32 at
+// a time 26.6 (16: 41); 64 rows 64 at a time 33.0 against 41.8 for 32, but 18.6 against 12.4 at N = K = 4096.
+template <bool ALIGNED, typename O> int gemm_f8_rows(hipStream_t st, const F8Args &a) {
+    const bool wide = a.N >= 32 * 256; // a work-group of 32 columns for each unit
+    if (a.M <= 16) return wide ? gemm_f8_rows_launch<ALIGNED, O, 1, 2, ALIGNED ? 4 : 2, 16>(st, a) : gemm_f8_rows_launch<ALIGNED, O, 1, 1, 4>(st, a);
+    if (a.M <= 32 || !wide) return gemm_f8_rows_launch<ALIGNED, O, 2, 2, 2>(st, a);
+    return gemm_f8_rows_launch<ALIGNED, O, 4, 2, 2>(st, a);
+}
+
+// Which tile: its launch's time by rounds of what is resident, from measured rounds of 64 blocks of k (us; 256 units) with one
+// work-group to a unit and with as many as fit.
+struct TileTime {
+    uint32_t m, n, per_unit;
+    float one, full;
+};
+uint32_t best_tile(const TileTime *t, uint32_t count, const F8Args &a) {
+    constexpr uint64_t UNITS = 256;
+    uint32_t best = 0;
+    float least = 0.f;
+    for (uint32_t i = 0; i < count; ++i) {
+        const uint64_t tiles = (uint64_t)((a.M + t[i].m - 1) / t[i].m) * ((a.N + t[i].n - 1) / t[i].n), round = UNITS * t[i].per_unit;
+        const uint64_t rest = tiles % round;
+        const float time = (float)(tiles / round) * t[i].full + (rest == 0 ? 0.f : rest <= UNITS ? t[i].one : t[i].full);
+        if (i == 0 || time < least) {
+            best = i;
+            least = time;
+        }
+    }
+    return best;
+}
+
 template <typename O> int gemm_f8_launch(wk_stream *s, const F8Args &a, bool aligned) {
-    if (a.M <= 64) return aligned ? gemm_f8_rows_launch<true, O>(s->stream, a) : gemm_f8_rows_launch<false, O>(s->stream, a);
-    // lane offsets within a tile are 32 bits
-    if (aligned && a.lda < (1u << 23) && a.ldb < (1u << 23) && a.sap < (1u << 21) && a.sbp < (1u << 21)) {
+    const hipStream_t st = s->stream;
+    // the loads into LDS have lane offsets of 32 bits within a tile
+    const bool direct = aligned && a.lda < (1u << 23) && a.ldb < (1u << 23) && a.sap < (1u << 21) && a.sbp < (1u << 21);
+    // f32 results: 64 rows 33 us either way (N = K = 8192); 16-bit ones have tiles of 8-bit instructions from 17 rows on (64: 20 us, 32 rows in the
+    // lanes 26)
+    if (a.M <= (direct && !std::is_same_v<O, float> ? 16 : 64)) return aligned ? gemm_f8_rows<true, O>(st, a) : gemm_f8_rows<false, O>(st, a);
+    if (direct) {
         if constexpr (std::is_same_v<O, float>) {
-            return gemm_f8_dma_launch<O, 2, 2, 4, 4>(s->stream, a);
+            constexpr TileTime t[] = {{128, 128, 2, 76, 145}, {64, 128, 2, 51, 82}, {64, 64, 2, 35, 48}};
+            switch (best_tile(t, 3, a)) {
+            case 0: return gemm_f8_dma_launch<O, 2, 2, 4, 4, 2>(st, a);
+            case 1: return gemm_f8_dma_launch<O, 2, 2, 2, 4, 3>(st, a);
+            default: return gemm_f8_dma_launch<O, 2, 2, 2, 2, 4>(st, a);
+            }
         } else {
-            if ((uint64_t)a.M * a.N >= (uint64_t)256 * 256 * 200) return gemm_f8_dma_launch<O, 2, 4, 8, 4>(s->stream, a);
-            return gemm_f8_dma_launch<O, 2, 2, 4, 4>(s->stream, a);
+            constexpr TileTime t[] = {{256, 256, 1, 147, 147}, {128, 128, 2, 46, 88}, {64, 128, 2, 29, 51}, {64, 64, 2, 21, 33}};
+            switch (best_tile(t, 4, a)) {
+            case 0: return gemm_f8_dma_launch<O, 2, 4, 8, 4, 2>(st, a);
+            case 1: return gemm_f8_dma_launch<O, 2, 2, 4, 4, 2>(st, a);
+            case 2: return gemm_f8_dma_launch<O, 2, 2, 2, 4, 3>(st, a);
+            default: return gemm_f8_dma_launch<O, 2, 2, 2, 2, 4>(st, a);
+            }
         }
     }
     const uint64_t tiles = (uint64_t)((a.M + 127) / 128) * ((a.N + 127) / 128);
     if (tiles > 0x7fffffffull) return WK_E_INVALID_VALUE;
     if (aligned)
-        hipLaunchKernelGGL((gemm_f8_tile_kernel<true, O>), dim3((unsigned)tiles), dim3(256), 0, s->stream, a);
+        hipLaunchKernelGGL((gemm_f8_tile_kernel<true, O>), dim3((unsigned)tiles), dim3(256), 0, st, a);
     else
-        hipLaunchKernelGGL((gemm_f8_tile_kernel<false, O>), dim3((unsigned)tiles), dim3(256), 0, s->stream, a);
+        hipLaunchKernelGGL((gemm_f8_tile_kernel<false, O>), dim3((unsigned)tiles), dim3(256), 0, st, a);
     return launch_status();
 }
 
