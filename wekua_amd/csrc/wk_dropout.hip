@@ -44,16 +44,19 @@ struct DropArgs {
     bool none; // p = 1: nothing is kept
 };
 
-// One thread takes PER consecutive elements of a row.  PHASE0: every row begins at a multiple of four elements, so the
-// PER words are whole blocks; otherwise a row's first word is (row * cols) % 4 words into its block and one block
-// more is drawn.
-template <typename T, int PER, bool PHASE0>
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2))); // 16 bytes at any element's address
+
+// One thread takes PER consecutive elements of a row, 16 bytes (f64: 32), loaded before their words are drawn.  PHASE0: every row
+// begins at a multiple of four elements, so the PER words are whole blocks; otherwise a row's first word is
+// (row * cols) % 4 words into its block and one block more is drawn.  STREAM: the tensors are more than the last-level cache
+// holds (256 MB) and pass it by.
+template <typename T, int PER, bool PHASE0, bool STREAM>
 __global__ __launch_bounds__(256) void dropout_kernel(const T *x, T *y, DropArgs a, typename wide_of<T>::type scale, uint64_t chunks_per_row,
                                                       uint64_t chunks) {
     using W = typename wide_of<T>::type;
+    constexpr int LOADS = PER * sizeof(T) / 16;
     const uint64_t idx = blockIdx.x * 256ull + threadIdx.x;
     if (idx >= chunks) return;
-    const uint64_t count = a.offset + (a.step ? *a.step : 0);
     uint64_t row = 0, c = idx * PER;
     if (a.total_rows > 1) {
         row = (chunks >> 32) ? idx / chunks_per_row : (uint32_t)idx / (uint32_t)chunks_per_row;
@@ -66,6 +69,21 @@ __global__ __launch_bounds__(256) void dropout_kernel(const T *x, T *y, DropArgs
     }
     const T *xp = x + slice * a.xsp + r * a.xrp + c;
     T *yp = y + slice * a.ysp + r * a.yrp + c;
+    T v[PER];
+    const bool whole = c + PER <= a.cols;
+    if (whole) {
+        u32x4_any raw[LOADS];
+#pragma unroll
+        for (int l = 0; l < LOADS; ++l) {
+            const u32x4_any *from = reinterpret_cast<const u32x4_any *>(xp) + l;
+            raw[l] = STREAM ? __builtin_nontemporal_load(from) : *from;
+        }
+        __builtin_memcpy(v, raw, sizeof v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < PER; ++e) v[e] = c + e < a.cols ? xp[e] : T(0);
+    }
+    const uint64_t count = a.offset + (a.step ? *a.step : 0);
     const uint64_t first = row * a.cols + c;
     constexpr int BLOCKS = PER / 4 + (PHASE0 ? 0 : 1);
     uint32_t w[BLOCKS * 4];
@@ -82,23 +100,28 @@ __global__ __launch_bounds__(256) void dropout_kernel(const T *x, T *y, DropArgs
 #pragma unroll
             for (int e = 0; e + s < BLOCKS * 4; ++e) w[e] = phase & s ? w[e + s] : w[e];
     }
-    T v[PER];
-    const bool whole = c + PER <= a.cols;
-    if (whole) {
-        __builtin_memcpy(v, xp, sizeof v);
-    } else {
-#pragma unroll
-        for (int e = 0; e < PER; ++e) v[e] = c + e < a.cols ? xp[e] : T(0);
-    }
 #pragma unroll
     for (int e = 0; e < PER; ++e) v[e] = w[e] >= a.threshold && !a.none ? (T)((W)v[e] * scale) : T(0);
     if (whole) {
-        __builtin_memcpy(yp, v, sizeof v);
+        u32x4_any raw[LOADS];
+        __builtin_memcpy(raw, v, sizeof v);
+#pragma unroll
+        for (int l = 0; l < LOADS; ++l) {
+            u32x4_any *to = reinterpret_cast<u32x4_any *>(yp) + l;
+            if (STREAM) __builtin_nontemporal_store(raw[l], to);
+            else *to = raw[l];
+        }
     } else {
 #pragma unroll
         for (int e = 0; e < PER; ++e)
             if (c + e < a.cols) yp[e] = v[e];
     }
+}
+
+template <typename T, int PER, bool PHASE0, bool STREAM>
+void dropout_enqueue(hipStream_t st, uint64_t chunks, uint64_t per_row, const void *x, void *y, const DropArgs &a, typename wide_of<T>::type scale) {
+    hipLaunchKernelGGL((dropout_kernel<T, PER, PHASE0, STREAM>), dim3((unsigned)((chunks + 255) / 256)), dim3(256), 0, st, static_cast<const T *>(x),
+                       static_cast<T *>(y), a, scale, per_row, chunks);
 }
 
 template <typename T> int dropout_launch(wk_stream *s, const void *x, void *y, DropArgs a, double p) {
@@ -113,13 +136,9 @@ template <typename T> int dropout_launch(wk_stream *s, const void *x, void *y, D
     const W scale = p < 1.0 ? (W)(1.0 / (1.0 - p)) : W(0);
     const uint64_t per_row = (a.cols + PER - 1) / PER, chunks = per_row * a.total_rows;
     if ((chunks + 255) / 256 > 0x7fffffffull) return WK_E_INVALID_VALUE;
-    const dim3 grid((unsigned)((chunks + 255) / 256));
-    if (a.total_rows == 1 || a.cols % 4 == 0)
-        hipLaunchKernelGGL((dropout_kernel<T, PER, true>), grid, dim3(256), 0, s->stream, static_cast<const T *>(x), static_cast<T *>(y), a,
-                           scale, per_row, chunks);
-    else
-        hipLaunchKernelGGL((dropout_kernel<T, PER, false>), grid, dim3(256), 0, s->stream, static_cast<const T *>(x), static_cast<T *>(y), a,
-                           scale, per_row, chunks);
+    const bool phase0 = a.total_rows == 1 || a.cols % 4 == 0, stream = 2 * a.total_rows * a.cols * sizeof(T) > (256ull << 20);
+    if (phase0) (stream ? dropout_enqueue<T, PER, true, true> : dropout_enqueue<T, PER, true, false>)(s->stream, chunks, per_row, x, y, a, scale);
+    else (stream ? dropout_enqueue<T, PER, false, true> : dropout_enqueue<T, PER, false, false>)(s->stream, chunks, per_row, x, y, a, scale);
     return launch_status();
 }
 

@@ -146,6 +146,8 @@ template <typename O> __device__ __forceinline__ O nth_order(O order, uint32_t t
     return t;
 }
 
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2))); // 16 bytes at any element's address
+
 template <typename T, int N> __device__ __forceinline__ void load_n(const T *p, uint32_t left, T raw[N]) {
     if (left >= (uint32_t)N) {
         __builtin_memcpy(raw, p, sizeof(T) * N);
@@ -501,7 +503,7 @@ int logprobs_launch(wk_stream *s, uint64_t rows, uint32_t vocab, const void *log
     return launch_status();
 }
 
-constexpr int GRAD_DEEP = 4;
+constexpr int GRAD_DEEP = 2;
 
 template <typename A> struct GradArgs {
     const A *lse, *entropy, *w, *h;
@@ -509,8 +511,11 @@ template <typename A> struct GradArgs {
     bool wide_targets;
 };
 
-// One thread takes DEEP x 16 bytes of a row, all loads issued before any is used; blockIdx.x counts a row's segments first.
-template <typename T, bool ENTROPY>
+// One thread takes GRAD_DEEP x 16 bytes of a row, all loads issued before any is used; blockIdx.x counts a row's segments first.
+// STREAM: both tensors together are more than the last-level cache holds (256 MB), so that neither is kept there: 4096 x 65536 bf16
+// 190 -> 171 us (6.3 TB/s), where 1000 x 32003 f32, which it half holds, loses (39 -> 45).  Two loads in flight per thread did
+// better than one, four and eight (171 against 175, 180 and 185).
+template <typename T, bool ENTROPY, bool STREAM>
 __global__ __launch_bounds__(256) void logprobs_grad_kernel(const T *x, uint64_t pitch, T *dx, uint64_t grad_pitch, uint32_t vocab,
                                                             uint32_t segments, GradArgs<typename stat_of<T>::type> a) {
     using A = typename stat_of<T>::type;
@@ -524,7 +529,12 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(const T *x, uint64_t
 #pragma unroll
     for (int u = 0; u < GRAD_DEEP; ++u) {
         const uint32_t c = c0 + u * 256 * VE;
-        load_n<T, VE>(xr + (c < vocab ? c : 0), c < vocab ? vocab - c : 0, raw[u]);
+        if (STREAM && c < vocab && vocab - c >= (uint32_t)VE) {
+            const u32x4_any v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any *>(xr + c));
+            __builtin_memcpy(raw[u], &v, 16);
+        } else {
+            load_n<T, VE>(xr + (c < vocab ? c : 0), c < vocab ? vocab - c : 0, raw[u]);
+        }
     }
     const A lse = a.lse[row];
     A w = A(0), h = A(0), ent = A(0);
@@ -552,7 +562,11 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(const T *x, uint64_t
             raw[u][e] = (T)(empty ? A(0) : g);
         }
         if (vocab - c >= (uint32_t)VE) {
-            __builtin_memcpy(dr + c, raw[u], 16);
+            u32x4_any v;
+            __builtin_memcpy(&v, raw[u], 16);
+            u32x4_any *to = reinterpret_cast<u32x4_any *>(dr + c);
+            if (STREAM) __builtin_nontemporal_store(v, to);
+            else *to = v;
         } else {
 #pragma unroll
             for (int e = 0; e < VE; ++e)
@@ -561,17 +575,22 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(const T *x, uint64_t
     }
 }
 
+template <typename T, bool ENTROPY, bool STREAM>
+void grad_enqueue(hipStream_t st, uint64_t rows, uint32_t vocab, const void *x, uint64_t pitch, void *dx, uint64_t grad_pitch, uint32_t segments,
+                  const GradArgs<typename stat_of<T>::type> &a) {
+    hipLaunchKernelGGL((logprobs_grad_kernel<T, ENTROPY, STREAM>), dim3((unsigned)(rows * segments)), dim3(256), 0, st,
+                       static_cast<const T *>(x), pitch, static_cast<T *>(dx), grad_pitch, vocab, segments, a);
+}
+
 template <typename T>
 int grad_launch(wk_stream *s, uint64_t rows, uint32_t vocab, const void *x, uint64_t pitch, void *dx, uint64_t grad_pitch,
                 const GradArgs<typename stat_of<T>::type> &a) {
     constexpr uint32_t step = 256 * GRAD_DEEP * 16 / sizeof(T);
     const uint32_t segments = (vocab + step - 1) / step;
     if (rows * segments > 0x7fffffffull) return WK_E_INVALID_VALUE;
-    const dim3 grid((unsigned)(rows * segments));
-    if (a.h)
-        hipLaunchKernelGGL((logprobs_grad_kernel<T, true>), grid, dim3(256), 0, s->stream, static_cast<const T *>(x), pitch, static_cast<T *>(dx), grad_pitch, vocab, segments, a);
-    else
-        hipLaunchKernelGGL((logprobs_grad_kernel<T, false>), grid, dim3(256), 0, s->stream, static_cast<const T *>(x), pitch, static_cast<T *>(dx), grad_pitch, vocab, segments, a);
+    const bool stream = 2 * rows * vocab * sizeof(T) > (256ull << 20);
+    if (a.h) (stream ? grad_enqueue<T, true, true> : grad_enqueue<T, true, false>)(s->stream, rows, vocab, x, pitch, dx, grad_pitch, segments, a);
+    else (stream ? grad_enqueue<T, false, true> : grad_enqueue<T, false, false>)(s->stream, rows, vocab, x, pitch, dx, grad_pitch, segments, a);
     return launch_status();
 }
 
