@@ -28,10 +28,18 @@ __device__ __forceinline__ float larger(float a, float b) {
     return __uint_as_float(x > y ? x : y);
 }
 
-template <typename T> __device__ __forceinline__ void load8(const T *p, uint64_t left, float v[PER]) {
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2))); // 16 bytes at any element's address
+
+template <bool STREAM, typename T> __device__ __forceinline__ void load8(const T *p, uint64_t left, float v[PER]) {
     T raw[PER];
     if (left >= PER) {
-        __builtin_memcpy(raw, p, sizeof raw);
+        u32x4_any w[sizeof raw / 16];
+#pragma unroll
+        for (uint32_t i = 0; i < sizeof raw / 16; ++i) {
+            const u32x4_any *from = reinterpret_cast<const u32x4_any *>(p) + i;
+            w[i] = STREAM ? __builtin_nontemporal_load(from) : *from;
+        }
+        __builtin_memcpy(raw, w, sizeof raw);
     } else {
 #pragma unroll
         for (int e = 0; e < PER; ++e) raw[e] = (uint64_t)e < left ? p[e] : T(0);
@@ -62,7 +70,8 @@ __device__ __forceinline__ void store8(uint8_t *p, uint64_t left, const float v[
     }
 }
 
-// One scale per row and 128 columns: sixteen lanes to a block, sixteen blocks to a work-group.
+// One scale per row and 128 columns: sixteen lanes to a block, sixteen blocks to a work-group.  Bound by memory: 8192 x 8192 f32
+// 58 us (5.8 TB/s), bf16 41.
 template <typename T>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T *__restrict__ x, uint64_t pitch, uint64_t rows, uint64_t cols,
                                                             uint8_t *__restrict__ q, uint64_t q_pitch, float *__restrict__ scales,
@@ -73,7 +82,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T *__restrict_
     const uint64_t row = in ? blk / col_blocks : 0, cb = in ? blk - row * col_blocks : 0;
     const uint64_t c = cb * KB + lane * PER, left = in && c < cols ? cols - c : 0;
     float v[PER], amax = 0.f;
-    load8(x + row * pitch + (left ? c : 0), left, v);
+    load8<false>(x + row * pitch + (left ? c : 0), left, v);
 #pragma unroll
     for (int e = 0; e < PER; ++e) amax = larger(amax, __builtin_fabsf(v[e]));
 #pragma unroll
@@ -84,8 +93,11 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T *__restrict_
     if (in && lane == 0) scales[row * scale_pitch + cb] = scale;
 }
 
-// One scale per 128 x 128 block: a work-group holds the block in registers, 8 columns of every 16th row to a thread.
-template <typename T>
+// One scale per 128 x 128 block: a work-group holds the block in registers, 8 columns of every 16th row to a thread.  Bound by
+// memory: 8192 x 8192 f32 58 us (5.8 TB/s), bf16 36.  STREAM: the last-level cache (256 MB) would not hold x and what
+// comes next, so x passes it by (bf16 44 -> 36 us; 4096 x 4096 f32, which it holds, 15 -> 19).  Four blocks side by side
+// to a work-group of 1024 threads, for longer runs of memory, were slower (74 us).
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(256) void quantize_blocks_kernel(const T *__restrict__ x, uint64_t pitch, uint64_t rows, uint64_t cols,
                                                               uint8_t *__restrict__ q, uint64_t q_pitch, float *__restrict__ scales,
                                                               uint64_t scale_pitch, uint64_t col_blocks) {
@@ -98,7 +110,7 @@ __global__ __launch_bounds__(256) void quantize_blocks_kernel(const T *__restric
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
         const uint64_t r = r0 + i * STEP, l = r < rows ? left : 0;
-        load8(x + (l ? r * pitch + c : 0), l, v[i]);
+        load8<STREAM>(x + (l ? r * pitch + c : 0), l, v[i]);
 #pragma unroll
         for (int e = 0; e < PER; ++e) amax = larger(amax, __builtin_fabsf(v[i][e]));
     }
@@ -126,9 +138,12 @@ int quantize_launch(wk_stream *s, uint64_t rows, uint64_t cols, const void *x, u
     if (block_rows == 1)
         hipLaunchKernelGGL(quantize_rows_kernel<T>, dim3((unsigned)groups), dim3(256), 0, s->stream, static_cast<const T *>(x), pitch, rows,
                            cols, static_cast<uint8_t *>(q), q_pitch, scales, scale_pitch, col_blocks);
+    else if (rows * cols * sizeof(T) > (128ull << 20))
+        hipLaunchKernelGGL((quantize_blocks_kernel<T, true>), dim3((unsigned)groups), dim3(256), 0, s->stream, static_cast<const T *>(x), pitch,
+                           rows, cols, static_cast<uint8_t *>(q), q_pitch, scales, scale_pitch, col_blocks);
     else
-        hipLaunchKernelGGL(quantize_blocks_kernel<T>, dim3((unsigned)groups), dim3(256), 0, s->stream, static_cast<const T *>(x), pitch, rows,
-                           cols, static_cast<uint8_t *>(q), q_pitch, scales, scale_pitch, col_blocks);
+        hipLaunchKernelGGL((quantize_blocks_kernel<T, false>), dim3((unsigned)groups), dim3(256), 0, s->stream, static_cast<const T *>(x), pitch,
+                           rows, cols, static_cast<uint8_t *>(q), q_pitch, scales, scale_pitch, col_blocks);
     return launch_status();
 }
 
