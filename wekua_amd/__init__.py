@@ -31,7 +31,7 @@ import numpy as np
 
 from . import _capi
 from ._capi import WkError as WekuaError  # noqa: F401  (re-export)
-from .raw import DTYPE_NAMES, dtype_id, elem_size, is_complex, real_np_dtype, scalar_bytes
+from .raw import DTYPE_NAMES, EXTRA_DTYPES, dtype_id, elem_size, is_complex, real_np_dtype, scalar_bytes
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 HOST_LIB_PATH = os.path.join(_PKG, "libwekua_host.so")
@@ -119,6 +119,21 @@ HOST_SIGNATURES = {
     "wkz_nn_optimizer_step": (ci, [vp, vp, vp]),
     "wkz_nn_optimizer_zero": (ci, [vp, vp]),
     "wkz_nn_optimizer_deinit": (ci, [vp, vp]),
+    # the token end of a network
+    "wkz_random_dropout": (ci, [vp, vp, vp, ctypes.c_double, u64, u64, vp]),
+    "wkz_block_scaled_init": (ci, [vp, vp, u64, u64, u64, ctypes.POINTER(vp)]),
+    "wkz_block_scaled_deinit": (ci, [vp, vp]),
+    "wkz_block_scaled_quantize": (ci, [vp, vp, vp]),
+    "wkz_block_scaled_tensor": (ci, [vp, ci, ctypes.POINTER(vp)]),
+    "wkz_gemm_f8": (ci, [vp, vp, vp, vp, ci, vp]),
+    "wkz_nn_dropout_init": (ci, [vp, ci, u64, ctypes.c_double, u64p, ctypes.POINTER(vp)]),
+    "wkz_nn_layer_set_training": (ci, [vp, ci]),
+    "wkz_nn_token_logprobs_init": (ci, [vp, vp, ci, u64, u64, ctypes.c_uint32, ctypes.POINTER(vp)]),
+    "wkz_nn_token_logprobs_deinit": (ci, [vp, vp]),
+    "wkz_nn_token_logprobs_tensor": (ci, [vp, ci, ctypes.POINTER(vp)]),
+    "wkz_nn_token_logprobs_forward": (ci, [vp, vp, vp, vp]),
+    "wkz_nn_token_logprobs_backward": (ci, [vp, vp, vp, vp, vp, vp, vp]),
+    "wkz_nn_loss_tokens": (ci, [ci, vp, vp, vp, vp, vp, vp]),
 }
 
 _host = None
@@ -161,7 +176,7 @@ class CommandQueue:
         self.wekua_id = index
 
     def isTypeSupported(self, dtype: str) -> bool:
-        return dtype in DTYPE_NAMES
+        return dtype in DTYPE_NAMES or dtype in EXTRA_DTYPES
 
 
 class Context:
@@ -392,6 +407,12 @@ class random:
         _check(_lib().wkz_random_uniform(pipeline._h, tensor._h, seed_arg, pmin, pmax), "random.uniform")
 
     @staticmethod
+    def dropout(pipeline: Pipeline, x: Tensor, y: Tensor, p: float, seed: int, offset: int = 0, step: "Tensor | None" = None) -> None:
+        """y = x / (1 - p) where an element is kept, else 0 (y may be x); the same call on the gradient is the backward pass.
+        `step`: a one-element u64 tensor that is added to `offset` when the kernel runs.  f32, f64, f16, bf16."""
+        _check(_lib().wkz_random_dropout(pipeline._h, x._h, y._h, float(p), seed, offset, step._h if step is not None else None), "random.dropout")
+
+    @staticmethod
     def hash(index: int, seed: int) -> int:
         """The 64-bit hash random.uniform draws from."""
         return int(_capi.load().wk_random_hash(index, seed))
@@ -457,7 +478,52 @@ class GemmPackedTensors:
         _check(_lib().wkz_packed_pack(self._h, pipeline._h, a._h, int(op_a), b._h, int(op_b)), "GemmPackedTensors.pack")
 
 
+class BlockScaled:
+    """A matrix as 8-bit codes (`codes`, dtype f8e4m3: numpy uint8) with one f32 scale (`scales`) for each block of
+    block_rows (1: activations, 128: weights) x 128 elements.  No counterpart in the reference."""
+
+    def __init__(self, handle, context):
+        self._h = handle
+        self.context = context
+
+    @classmethod
+    def init(cls, context: Context, pipeline: Pipeline, rows: int, cols: int, block_rows: int) -> "BlockScaled":
+        h = vp()
+        _check(_lib().wkz_block_scaled_init(context._h, pipeline._h, rows, cols, block_rows, ctypes.byref(h)), "BlockScaled.init")
+        return cls(h, context)
+
+    def deinit(self, pipeline: Pipeline) -> None:
+        if self._h:
+            _check(_lib().wkz_block_scaled_deinit(self._h, pipeline._h), "BlockScaled.deinit")
+            self._h = None
+
+    def quantize(self, pipeline: Pipeline, x: Tensor) -> None:
+        """Codes and scales of x (f32, f16, bf16) of the same shape."""
+        _check(_lib().wkz_block_scaled_quantize(self._h, pipeline._h, x._h), "BlockScaled.quantize")
+
+    def _tensor(self, which: int, dtype: str) -> Tensor:
+        h = vp()
+        _check(_lib().wkz_block_scaled_tensor(self._h, which, ctypes.byref(h)), "BlockScaled")
+        return Tensor._borrow(h, dtype, self.context)
+
+    @property
+    def codes(self) -> Tensor:
+        return self._tensor(0, "f8e4m3")
+
+    @property
+    def scales(self) -> Tensor:
+        return self._tensor(1, "f32")
+
+
 class blas:
+    BlockScaled = BlockScaled
+
+    @staticmethod
+    def gemmF8(pipeline: Pipeline, a: BlockScaled, b: BlockScaled, bias: "Tensor | None", kind: int, c: Tensor) -> None:
+        """c = act(a b^T + bias): a {M, K} with block_rows 1, b {N, K} with block_rows 128, c {M, N} of f32, f16 or bf16;
+        kind: -1 none, 0 sigmoid, 1 tanh."""
+        _check(_lib().wkz_gemm_f8(pipeline._h, a._h, b._h, bias._h if bias is not None else None, int(kind), c._h), "blas.gemmF8")
+
     class Operation(enum.IntEnum):
         no_transpose = 0
         transpose = 1
@@ -501,4 +567,4 @@ from . import nn  # noqa: E402  (needs the classes above)
 from .nn import math  # noqa: E402,F401
 
 __all__ = ["nn", "math", "printZ", "print_tensor", "transpose", "random", "convertions", "Space", "Context", "Pipeline", "Tensor", "CommandQueue", "DeviceType", "memory", "fill", "identity", "blas",
-           "GemmPackedTensors", "WekuaError", "DTYPE_NAMES", "dtype_id", "elem_size", "is_complex", "real_np_dtype"]
+           "GemmPackedTensors", "BlockScaled", "WekuaError", "EXTRA_DTYPES", "DTYPE_NAMES", "dtype_id", "elem_size", "is_complex", "real_np_dtype"]

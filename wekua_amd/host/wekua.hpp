@@ -68,6 +68,21 @@ template <typename R> struct Complex {
     R real, imag;
 };
 
+// Element formats beyond the reference's twenty, as their bits: storage for the operators that take them
+// (random::dropout, blas::gemmF8, nn::TokenLogProbs); everything else answers TypeNotSupported or does not instantiate.
+struct F16 {
+    uint16_t bits;
+};
+struct BF16 {
+    uint16_t bits;
+};
+struct F8E4M3 {
+    uint8_t bits;
+};
+template <typename T> constexpr bool isExtraFormat() {
+    return std::is_same_v<T, F16> || std::is_same_v<T, BF16> || std::is_same_v<T, F8E4M3>;
+}
+
 template <typename T> struct is_complex : std::false_type {};
 template <typename R> struct is_complex<Complex<R>> : std::true_type {};
 template <typename T> struct scalar_of { using type = T; };
@@ -92,7 +107,12 @@ template <typename T> constexpr int getTypeId() {
     else static_assert(sizeof(R) == 0, "Type not supported");
 }
 // getTypeIndex: 0..19 (types.zig:60-86); also the dtype id of the C ABI
-template <typename T> constexpr int getTypeIndex() { return getTypeId<T>() + (isComplex<T>() ? 10 : 0); }
+template <typename T> constexpr int getTypeIndex() {
+    if constexpr (std::is_same_v<T, F16>) return WK_F16;
+    else if constexpr (std::is_same_v<T, BF16>) return WK_BF16;
+    else if constexpr (std::is_same_v<T, F8E4M3>) return WK_F8E4M3;
+    else return getTypeId<T>() + (isComplex<T>() ? 10 : 0);
+}
 
 template <typename T> constexpr T getOne() {
     if constexpr (isComplex<T>()) return T{1, 0};
@@ -120,6 +140,10 @@ struct CommandQueue {
     uint32_t vector_widths[10] = {16, 16, 8, 8, 4, 4, 2, 2, 4, 2};
 
     template <typename T> bool isTypeSupported() const { return true; }
+    template <typename T> uint32_t vectorWidth() const {
+        if constexpr (isExtraFormat<T>()) return 16 / sizeof(T);
+        else return vector_widths[getTypeId<T>()];
+    }
 };
 
 struct Context {
@@ -288,7 +312,7 @@ template <typename T> struct Tensor {
 
         constexpr bool cplx = core::isComplex<T>();
         const bool vectors_enabled = !cplx && config.vectors_enabled;
-        const uint64_t vw = vectors_enabled ? context->command_queues[0].vector_widths[core::getTypeId<T>()] : 1;
+        const uint64_t vw = vectors_enabled ? context->command_queues[0].template vectorWidth<T>() : 1;
         t->flags.vectors_enabled = vectors_enabled && vw > 1;
 
         const uint64_t cols = shape.back();
@@ -505,6 +529,20 @@ void uniform(Pipeline *pipeline, Tensor<T> *tensor, std::optional<uint64_t> seed
     check(wk_random_uniform(pipeline->command_queue->stream, core::getTypeIndex<T>(), shape3, tensor->buffer,
                             tensor->memory_layout.row_pitch, tensor->memory_layout.slice_pitch, global_seed,
                             range_defined ? &mn : nullptr, range_defined ? &range : nullptr));
+    pipeline->append(1);
+}
+
+// No counterpart in the reference.  y = x / (1 - p) where an element is kept, 0 elsewhere; y may be x.  The mask is a function
+// of (seed, offset + *step, element): the same call on the gradient is the backward pass.  step: one element in device
+// memory that is read when the kernel runs, or null.  f32, f64, F16, BF16.
+template <typename T>
+void dropout(Pipeline *pipeline, Tensor<T> *x, Tensor<T> *y, double p, uint64_t seed, uint64_t offset = 0, Tensor<uint64_t> *step = nullptr) {
+    helpers::eqlTensorsShape<T>(x, y);
+    if (x->context != y->context || (step && step->context != x->context)) throw Error(WK_E_UNQUAL_TENSORS_CONTEXT);
+    const uint64_t shape3[3] = {x->depth(), x->rows(), x->cols()};
+    check(wk_dropout(pipeline->command_queue->stream, core::getTypeIndex<T>(), shape3, x->buffer, x->memory_layout.row_pitch,
+                     x->memory_layout.slice_pitch, y->buffer, y->memory_layout.row_pitch, y->memory_layout.slice_pitch, p, seed, offset,
+                     step ? static_cast<const uint64_t *>(step->buffer) : nullptr));
     pipeline->append(1);
 }
 } // namespace random
@@ -898,6 +936,60 @@ void gemm(Pipeline *pipeline, std::optional<T> alpha, Tensor<T> *a, Operation op
         else packed_tensors->recordB(b, op_b, stream, alpha);
     }
     check(rc);
+    pipeline->append(1);
+}
+
+// ---- products of 8-bit floating point (no counterpart in the reference) ------------------------------
+// A matrix as 8-bit codes with one f32 scale for each block of block_rows (1: activations, 128: weights) x 128 elements.
+struct BlockScaled {
+    uint64_t block_rows = 1;
+    Tensor<core::F8E4M3> *codes = nullptr; // {rows, cols}
+    Tensor<float> *scales = nullptr;       // {ceil(rows / block_rows), ceil(cols / 128)}
+
+    static BlockScaled *init(const Context *context, Pipeline *pipeline, uint64_t rows, uint64_t cols, uint64_t block_rows) {
+        if (!rows || !cols || (block_rows != 1 && block_rows != 128)) throw Error(WK_E_INVALID_VALUE);
+        BlockScaled *b = new BlockScaled;
+        b->block_rows = block_rows;
+        try {
+            b->codes = Tensor<core::F8E4M3>::alloc(context, pipeline, {rows, cols});
+            b->scales = Tensor<float>::alloc(context, pipeline, {(rows + block_rows - 1) / block_rows, (cols + 127) / 128});
+        } catch (...) {
+            b->deinit(pipeline);
+            throw;
+        }
+        return b;
+    }
+    void deinit(Pipeline *pipeline) {
+        if (codes) codes->release(pipeline);
+        if (scales) scales->release(pipeline);
+        delete this;
+    }
+    // codes and scales of x (f32, F16 or BF16)
+    template <typename T> void quantize(Pipeline *pipeline, Tensor<T> *x) {
+        if (x->context != codes->context) throw Error(WK_E_UNQUAL_TENSORS_CONTEXT);
+        if (x->dimensions.shape != codes->dimensions.shape) throw Error(WK_E_UNQUAL_TENSORS_SHAPE);
+        check(wk_f8_quantize(pipeline->command_queue->stream, core::getTypeIndex<T>(), codes->rows(), codes->cols(), x->buffer,
+                             x->memory_layout.row_pitch, block_rows, codes->buffer, codes->memory_layout.row_pitch,
+                             static_cast<float *>(scales->buffer), scales->memory_layout.row_pitch));
+        pipeline->append(1);
+    }
+};
+
+// c = act(a b^T + bias): a {M, K} with a scale per row and block, b {N, K} with 128 x 128 blocks (a Linear's weights), c {M, N}
+// of f32, F16 or BF16; bias {N} or null; kind: WK_ACT_*.
+template <typename O>
+void gemmF8(Pipeline *pipeline, const BlockScaled *a, const BlockScaled *b, const Tensor<float> *bias, int kind, Tensor<O> *c) {
+    if (a->codes->context != b->codes->context || a->codes->context != c->context || (bias && bias->context != c->context))
+        throw Error(WK_E_UNQUAL_TENSORS_CONTEXT);
+    const auto &as = a->codes->dimensions.shape, &bs = b->codes->dimensions.shape, &cs = c->dimensions.shape;
+    if (a->block_rows != 1 || b->block_rows != 128 || cs.size() != 2) throw Error(WK_E_INVALID_VALUE);
+    if (as[1] != bs[1] || as[0] != cs[0] || bs[0] != cs[1]) throw Error(WK_E_INVALID_VALUE);
+    if (bias && bias->dimensions.shape != std::vector<uint64_t>{cs[1]}) throw Error(WK_E_UNQUAL_TENSORS_SHAPE);
+    check(wk_gemm_f8(pipeline->command_queue->stream, cs[0], cs[1], as[1], a->codes->buffer, a->codes->memory_layout.row_pitch,
+                     static_cast<const float *>(a->scales->buffer), a->scales->memory_layout.row_pitch, b->codes->buffer,
+                     b->codes->memory_layout.row_pitch, static_cast<const float *>(b->scales->buffer), b->scales->memory_layout.row_pitch,
+                     core::getTypeIndex<O>(), c->buffer, c->memory_layout.row_pitch, bias ? static_cast<const float *>(bias->buffer) : nullptr,
+                     kind));
     pipeline->append(1);
 }
 

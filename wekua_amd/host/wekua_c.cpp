@@ -100,6 +100,36 @@ template <typename F> void dispatch(int dtype, F &&f) {
     }
 }
 
+// element formats beyond the reference's twenty, and all of them together (what only stores or copies)
+template <typename F> bool dispatch_extra(int dtype, F &&f) {
+    switch (dtype) {
+    case WK_F16: f.template operator()<core::F16>(); return true;
+    case WK_BF16: f.template operator()<core::BF16>(); return true;
+    case WK_F8E4M3: f.template operator()<core::F8E4M3>(); return true;
+    default: return false;
+    }
+}
+template <typename F> void dispatch_any(int dtype, F &&f) {
+    if (!dispatch_extra(dtype, f)) dispatch(dtype, f);
+}
+// f32, f64, F16, BF16: what the operators on tokens take
+template <typename F> void dispatch_float(int dtype, F &&f) {
+    switch (dtype) {
+    case 8: f.template operator()<float>(); break;
+    case 9: f.template operator()<double>(); break;
+    case WK_F16: f.template operator()<core::F16>(); break;
+    case WK_BF16: f.template operator()<core::BF16>(); break;
+    default: throw Error(WK_E_TYPE_NOT_SUPPORTED);
+    }
+}
+// f32, F16, BF16: what the 8-bit operators read and return
+template <typename F> void dispatch_f8_side(int dtype, F &&f) {
+    if (dtype == WK_F32) f.template operator()<float>();
+    else if (dtype == WK_F16) f.template operator()<core::F16>();
+    else if (dtype == WK_BF16) f.template operator()<core::BF16>();
+    else throw Error(WK_E_TYPE_NOT_SUPPORTED);
+}
+
 template <typename T> std::optional<T> opt_scalar(const void *p) {
     if (!p) return std::nullopt;
     T v;
@@ -170,7 +200,7 @@ static int tensor_create(void *ctx, void *pipeline, int dtype, const uint64_t *s
         std::vector<uint64_t> shp(shape, shape + ndim);
         CreateConfig cfg;
         cfg.vectors_enabled = vectors_enabled != 0;
-        dispatch(dtype, [&]<typename T>() {
+        dispatch_any(dtype, [&]<typename T>() {
             Tensor<T> *t = zero ? Tensor<T>::alloc(static_cast<Context *>(ctx), static_cast<Pipeline *>(pipeline), shp, cfg)
                                 : Tensor<T>::empty(static_cast<Context *>(ctx), static_cast<Pipeline *>(pipeline), shp, cfg);
             *out = new TensorHandle{dtype, t};
@@ -186,14 +216,14 @@ int wkz_tensor_empty(void *ctx, void *pipeline, int dtype, const uint64_t *shape
 int wkz_tensor_release(void *tensor, void *pipeline) {
     return guard([&] {
         TensorHandle *h = static_cast<TensorHandle *>(tensor);
-        dispatch(h->dtype, [&]<typename T>() { static_cast<Tensor<T> *>(h->tensor)->release(static_cast<Pipeline *>(pipeline)); });
+        dispatch_any(h->dtype, [&]<typename T>() { static_cast<Tensor<T> *>(h->tensor)->release(static_cast<Pipeline *>(pipeline)); });
         delete h;
     });
 }
 int wkz_tensor_get_info(void *tensor, wkz_tensor_info *info) {
     return guard([&] {
         TensorHandle *h = static_cast<TensorHandle *>(tensor);
-        dispatch(h->dtype, [&]<typename T>() {
+        dispatch_any(h->dtype, [&]<typename T>() {
             const Tensor<T> *t = static_cast<Tensor<T> *>(h->tensor);
             std::memset(info, 0, sizeof *info);
             info->dtype = h->dtype;
@@ -221,7 +251,7 @@ int wkz_tensor_get_info(void *tensor, wkz_tensor_info *info) {
 int wkz_read_from_buffer(void *pipeline, void *tensor, const void *host, uint64_t len) {
     return guard([&] {
         TensorHandle *h = static_cast<TensorHandle *>(tensor);
-        dispatch(h->dtype, [&]<typename T>() {
+        dispatch_any(h->dtype, [&]<typename T>() {
             memory::readFromBuffer<T>(static_cast<Pipeline *>(pipeline), static_cast<Tensor<T> *>(h->tensor),
                                       static_cast<const T *>(host), (size_t)len);
         });
@@ -230,7 +260,7 @@ int wkz_read_from_buffer(void *pipeline, void *tensor, const void *host, uint64_
 int wkz_write_to_buffer(void *pipeline, void *tensor, void *host, uint64_t len) {
     return guard([&] {
         TensorHandle *h = static_cast<TensorHandle *>(tensor);
-        dispatch(h->dtype, [&]<typename T>() {
+        dispatch_any(h->dtype, [&]<typename T>() {
             memory::writeToBuffer<T>(static_cast<Pipeline *>(pipeline), static_cast<Tensor<T> *>(h->tensor),
                                      static_cast<T *>(host), (size_t)len);
         });
@@ -239,7 +269,7 @@ int wkz_write_to_buffer(void *pipeline, void *tensor, void *host, uint64_t len) 
 int wkz_fill_zeroes(void *pipeline, void *tensor) {
     return guard([&] {
         TensorHandle *h = static_cast<TensorHandle *>(tensor);
-        dispatch(h->dtype, [&]<typename T>() { fill::zeroes<T>(static_cast<Pipeline *>(pipeline), static_cast<Tensor<T> *>(h->tensor)); });
+        dispatch_any(h->dtype, [&]<typename T>() { fill::zeroes<T>(static_cast<Pipeline *>(pipeline), static_cast<Tensor<T> *>(h->tensor)); });
     });
 }
 int wkz_fill_one(void *pipeline, void *tensor) {
@@ -269,7 +299,7 @@ int wkz_memory_copy(void *pipeline, void *src, void *dst) {
     return guard([&] {
         TensorHandle *hs = static_cast<TensorHandle *>(src), *hd = static_cast<TensorHandle *>(dst);
         if (hs->dtype != hd->dtype) throw Error(WK_E_UNQUAL_TENSORS_ATTRIBUTE);
-        dispatch(hs->dtype, [&]<typename T>() {
+        dispatch_any(hs->dtype, [&]<typename T>() {
             memory::copy<T>(static_cast<Pipeline *>(pipeline), static_cast<Tensor<T> *>(hs->tensor), static_cast<Tensor<T> *>(hd->tensor));
         });
     });
@@ -298,7 +328,7 @@ int wkz_transpose(void *pipeline, void *result, void *tensor, uint64_t dim0, uin
     return guard([&] {
         TensorHandle *hr = static_cast<TensorHandle *>(result), *ht = static_cast<TensorHandle *>(tensor);
         if (hr->dtype != ht->dtype) throw Error(WK_E_UNQUAL_TENSORS_ATTRIBUTE);
-        dispatch(ht->dtype, [&]<typename T>() {
+        dispatch_any(ht->dtype, [&]<typename T>() {
             transpose<T>(static_cast<Pipeline *>(pipeline), static_cast<Tensor<T> *>(hr->tensor), static_cast<Tensor<T> *>(ht->tensor), dim0,
                          dim1);
         });
@@ -506,7 +536,7 @@ int wkz_nn_linear_init(void *ctx, void *pipeline, int dtype, uint64_t input, uin
                        int enable_bias, const uint64_t *seed, void **out) {
     return guard([&] {
         if (!out) throw Error(WK_E_INVALID_VALUE);
-        if (activation_kind != WK_ACT_NONE && activation_kind != WK_ACT_SIGMOID && activation_kind != WK_ACT_TANH)
+        if (activation_kind != WK_ACT_NONE && activation_kind != WK_ACT_SIGMOID && activation_kind != WK_ACT_TANH && activation_kind != nn::IDENTITY)
             throw Error(WK_E_INVALID_VALUE);
         dispatch_real(dtype, [&]<typename T>() {
             nn::ExtraParams extra;
@@ -700,6 +730,164 @@ int wkz_nn_optimizer_deinit(void *optimizer, void *pipeline) {
         OptimizerHandle *h = static_cast<OptimizerHandle *>(optimizer);
         dispatch_real(h->dtype, [&]<typename T>() { static_cast<nn::optimizers::Optimizer<T> *>(h->optimizer)->deinit(static_cast<Pipeline *>(pipeline)); });
         delete h;
+    });
+}
+
+// ---- the token end of a network -----------------------------------------------------------------------------
+int wkz_random_dropout(void *pipeline, void *x, void *y, double p, uint64_t seed, uint64_t offset, void *step) {
+    return guard([&] {
+        TensorHandle *hx = static_cast<TensorHandle *>(x), *hy = static_cast<TensorHandle *>(y), *hs = static_cast<TensorHandle *>(step);
+        if (hx->dtype != hy->dtype || (hs && hs->dtype != WK_U64)) throw Error(WK_E_UNQUAL_TENSORS_ATTRIBUTE);
+        dispatch_float(hx->dtype, [&]<typename T>() {
+            random::dropout<T>(static_cast<Pipeline *>(pipeline), static_cast<Tensor<T> *>(hx->tensor), static_cast<Tensor<T> *>(hy->tensor), p,
+                               seed, offset, hs ? static_cast<Tensor<uint64_t> *>(hs->tensor) : nullptr);
+        });
+    });
+}
+
+int wkz_block_scaled_init(void *ctx, void *pipeline, uint64_t rows, uint64_t cols, uint64_t block_rows, void **out) {
+    return guard([&] {
+        if (!out) throw Error(WK_E_INVALID_VALUE);
+        *out = blas::BlockScaled::init(static_cast<Context *>(ctx), static_cast<Pipeline *>(pipeline), rows, cols, block_rows);
+    });
+}
+int wkz_block_scaled_deinit(void *matrix, void *pipeline) {
+    return guard([&] { static_cast<blas::BlockScaled *>(matrix)->deinit(static_cast<Pipeline *>(pipeline)); });
+}
+int wkz_block_scaled_quantize(void *matrix, void *pipeline, void *x) {
+    return guard([&] {
+        TensorHandle *h = static_cast<TensorHandle *>(x);
+        dispatch_f8_side(h->dtype, [&]<typename T>() {
+            static_cast<blas::BlockScaled *>(matrix)->quantize<T>(static_cast<Pipeline *>(pipeline), static_cast<Tensor<T> *>(h->tensor));
+        });
+    });
+}
+// which: 0 codes, 1 scales; a borrowed handle, for wkz_tensor_handle_drop
+int wkz_block_scaled_tensor(void *matrix, int which, void **out) {
+    return guard([&] {
+        auto *b = static_cast<blas::BlockScaled *>(matrix);
+        if (!out || which < 0 || which > 1) throw Error(WK_E_INVALID_VALUE);
+        if (which == 0) *out = new TensorHandle{WK_F8E4M3, b->codes};
+        else *out = new TensorHandle{WK_F32, b->scales};
+    });
+}
+int wkz_gemm_f8(void *pipeline, void *a, void *b, void *bias, int kind, void *c) {
+    return guard([&] {
+        TensorHandle *hb = static_cast<TensorHandle *>(bias), *hc = static_cast<TensorHandle *>(c);
+        if (hb && hb->dtype != WK_F32) throw Error(WK_E_UNQUAL_TENSORS_ATTRIBUTE);
+        dispatch_f8_side(hc->dtype, [&]<typename O>() {
+            blas::gemmF8<O>(static_cast<Pipeline *>(pipeline), static_cast<blas::BlockScaled *>(a), static_cast<blas::BlockScaled *>(b),
+                            hb ? static_cast<Tensor<float> *>(hb->tensor) : nullptr, kind, static_cast<Tensor<O> *>(hc->tensor));
+        });
+    });
+}
+
+int wkz_nn_dropout_init(void *ctx, int dtype, uint64_t width, double p, const uint64_t *seed, void **out) {
+    return guard([&] {
+        if (!out) throw Error(WK_E_INVALID_VALUE);
+        dispatch_real(dtype, [&]<typename T>() {
+            nn::Layer<T> *l = nn::Dropout<T>::init(static_cast<Context *>(ctx), width, p, seed ? std::optional<uint64_t>(*seed) : std::nullopt);
+            *out = new LayerHandle{dtype, l};
+        });
+    });
+}
+int wkz_nn_layer_set_training(void *layer, int on) {
+    return guard([&] {
+        LayerHandle *h = static_cast<LayerHandle *>(layer);
+        dispatch_real(h->dtype, [&]<typename T>() { static_cast<nn::Layer<T> *>(h->layer)->setTraining(on != 0); });
+    });
+}
+
+struct TokenLogProbsHandle {
+    int dtype;
+    void *state; // nn::TokenLogProbs<T>*
+};
+int wkz_nn_token_logprobs_init(void *ctx, void *pipeline, int dtype, uint64_t rows, uint64_t vocab, uint32_t top, void **out) {
+    return guard([&] {
+        if (!out) throw Error(WK_E_INVALID_VALUE);
+        dispatch_float(dtype, [&]<typename T>() {
+            *out = new TokenLogProbsHandle{
+                dtype, nn::TokenLogProbs<T>::init(static_cast<Context *>(ctx), static_cast<Pipeline *>(pipeline), rows, vocab, top)};
+        });
+    });
+}
+int wkz_nn_token_logprobs_deinit(void *state, void *pipeline) {
+    return guard([&] {
+        auto *h = static_cast<TokenLogProbsHandle *>(state);
+        dispatch_float(h->dtype, [&]<typename T>() { static_cast<nn::TokenLogProbs<T> *>(h->state)->deinit(static_cast<Pipeline *>(pipeline)); });
+        delete h;
+    });
+}
+// which: 0 logprob, 1 lse, 2 entropy, 3 top_ids, 4 top_logprobs; NULL where there is none; for wkz_tensor_handle_drop
+int wkz_nn_token_logprobs_tensor(void *state, int which, void **out) {
+    return guard([&] {
+        auto *h = static_cast<TokenLogProbsHandle *>(state);
+        if (!out || which < 0 || which > 4) throw Error(WK_E_INVALID_VALUE);
+        dispatch_float(h->dtype, [&]<typename T>() {
+            auto *t = static_cast<nn::TokenLogProbs<T> *>(h->state);
+            void *list[5] = {t->logprob, t->lse, t->entropy, t->top_ids, t->top_logprobs};
+            const int stat = std::is_same_v<T, double> ? WK_F64 : WK_F32;
+            *out = list[which] ? new TensorHandle{which == 3 ? (int)WK_I32 : stat, list[which]} : nullptr;
+        });
+    });
+}
+int wkz_nn_token_logprobs_forward(void *state, void *pipeline, void *logits, void *targets) {
+    return guard([&] {
+        auto *h = static_cast<TokenLogProbsHandle *>(state);
+        TensorHandle *hl = static_cast<TensorHandle *>(logits), *ht = static_cast<TensorHandle *>(targets);
+        if (hl->dtype != h->dtype) throw Error(WK_E_UNQUAL_TENSORS_ATTRIBUTE);
+        if (ht && ht->dtype != WK_I32 && ht->dtype != WK_I64) throw Error(WK_E_TYPE_NOT_SUPPORTED);
+        dispatch_float(h->dtype, [&]<typename T>() {
+            auto *t = static_cast<nn::TokenLogProbs<T> *>(h->state);
+            auto *p = static_cast<Pipeline *>(pipeline);
+            auto *l = static_cast<Tensor<T> *>(hl->tensor);
+            if (ht && ht->dtype == WK_I64) t->forward(p, l, static_cast<const Tensor<int64_t> *>(ht->tensor));
+            else t->forward(p, l, ht ? static_cast<const Tensor<int32_t> *>(ht->tensor) : nullptr);
+        });
+    });
+}
+int wkz_nn_token_logprobs_backward(void *state, void *pipeline, void *logits, void *targets, void *logprob_grad, void *entropy_grad,
+                                   void *logits_grad) {
+    return guard([&] {
+        auto *h = static_cast<TokenLogProbsHandle *>(state);
+        TensorHandle *hl = static_cast<TensorHandle *>(logits), *ht = static_cast<TensorHandle *>(targets),
+                     *hw = static_cast<TensorHandle *>(logprob_grad), *he = static_cast<TensorHandle *>(entropy_grad),
+                     *hg = static_cast<TensorHandle *>(logits_grad);
+        const int stat = h->dtype == WK_F64 ? WK_F64 : WK_F32;
+        if (hl->dtype != h->dtype || hg->dtype != h->dtype || (hw && hw->dtype != stat) || (he && he->dtype != stat))
+            throw Error(WK_E_UNQUAL_TENSORS_ATTRIBUTE);
+        if (ht && ht->dtype != WK_I32 && ht->dtype != WK_I64) throw Error(WK_E_TYPE_NOT_SUPPORTED);
+        dispatch_float(h->dtype, [&]<typename T>() {
+            using S = typename nn::TokenLogProbs<T>::S;
+            auto *t = static_cast<nn::TokenLogProbs<T> *>(h->state);
+            auto *p = static_cast<Pipeline *>(pipeline);
+            auto *l = static_cast<Tensor<T> *>(hl->tensor), *g = static_cast<Tensor<T> *>(hg->tensor);
+            auto *w = hw ? static_cast<Tensor<S> *>(hw->tensor) : nullptr, *e = he ? static_cast<Tensor<S> *>(he->tensor) : nullptr;
+            if (ht && ht->dtype == WK_I64) t->backward(p, l, static_cast<const Tensor<int64_t> *>(ht->tensor), w, e, g);
+            else t->backward(p, l, ht ? static_cast<const Tensor<int32_t> *>(ht->tensor) : nullptr, w, e, g);
+        });
+    });
+}
+// host_error_result may be NULL (no mean is computed, nothing synchronises)
+int wkz_nn_loss_tokens(int calculate_derivative, void *pipeline, void *output, void *targets, void *state, void *cache,
+                       void *host_error_result) {
+    return guard([&] {
+        CacheHandle *hc = static_cast<CacheHandle *>(cache);
+        auto *hs = static_cast<TokenLogProbsHandle *>(state);
+        TensorHandle *ho = static_cast<TensorHandle *>(output), *ht = static_cast<TensorHandle *>(targets);
+        if (ho->dtype != hc->dtype || hs->dtype != hc->dtype) throw Error(WK_E_UNQUAL_TENSORS_ATTRIBUTE);
+        if (ht->dtype != WK_I32 && ht->dtype != WK_I64) throw Error(WK_E_TYPE_NOT_SUPPORTED);
+        dispatch_real(hc->dtype, [&]<typename T>() {
+            T result{};
+            auto run = [&](auto *t) {
+                nn::loss::tokens(calculate_derivative != 0, static_cast<Pipeline *>(pipeline), static_cast<Tensor<T> *>(ho->tensor), t,
+                                 static_cast<nn::TokenLogProbs<T> *>(hs->state), static_cast<nn::Cache<T> *>(hc->cache),
+                                 host_error_result ? &result : nullptr);
+            };
+            if (ht->dtype == WK_I64) run(static_cast<Tensor<int64_t> *>(ht->tensor));
+            else run(static_cast<Tensor<int32_t> *>(ht->tensor));
+            if (host_error_result) std::memcpy(host_error_result, &result, sizeof(T));
+        });
     });
 }
 

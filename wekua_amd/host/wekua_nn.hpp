@@ -9,6 +9,8 @@
 //   wekua::nn::Cache                    src/nn/layer/cache.zig
 //   wekua::nn::loss::mse                src/nn/loss/mse.zig:63-132
 //   wekua::nn::optimizers::GD           src/nn/optimizers/gd.zig (w += -lr * g through blas.axpy)
+//   wekua::nn::Identity, Dropout, TokenLogProbs, loss::tokens  no Zig counterpart: what training on tokens
+//                                       needs around the layers above
 //   wekua::nn::optimizers::Adam         no Zig counterpart (src/nn/optimizers/adam.zig is empty):
 //                                       textbook Adam, see wk_adam_step
 //
@@ -19,6 +21,7 @@
 // an optional seed.
 #pragma once
 
+#include <atomic>
 #include <chrono>
 #include <cmath>
 #include <limits>
@@ -73,10 +76,15 @@ template <typename T> T mean(Pipeline *pipeline, Tensor<T> *x) {
 namespace nn {
 
 // ---- activations ----------------------------------------------------------------------------
+// No counterpart in the reference, whose layers without an activation get zero gradients: the derivative is one.  The
+// activation of a last layer whose outputs are logits.
+constexpr int IDENTITY = 2;
+
 template <typename T> struct Activation {
     int kind = WK_ACT_NONE;
     // in place on the layer output (Activation.run)
     void run(Pipeline *pipeline, Tensor<T> *net_output) const {
+        if (kind == IDENTITY) return;
         const uint64_t shape3[3] = {net_output->depth(), net_output->rows(), net_output->cols()};
         check(wk_activation(pipeline->command_queue->stream, core::getTypeIndex<T>(), kind, shape3, net_output->buffer,
                             net_output->memory_layout.row_pitch, net_output->memory_layout.slice_pitch));
@@ -85,6 +93,7 @@ template <typename T> struct Activation {
     // derivative expressed through the activation output (Activation.getDerivative)
     void getDerivative(Pipeline *pipeline, Tensor<T> *output, Tensor<T> *derivative) const {
         helpers::eqlTensorsShape<T>(output, derivative);
+        if (kind == IDENTITY) return fill::one<T>(pipeline, derivative);
         const uint64_t shape3[3] = {output->depth(), output->rows(), output->cols()};
         check(wk_activation_dev(pipeline->command_queue->stream, core::getTypeIndex<T>(), kind, shape3, output->buffer,
                                 output->memory_layout.row_pitch, output->memory_layout.slice_pitch, derivative->buffer,
@@ -97,6 +106,9 @@ template <typename T> struct Sigmoid {
 };
 template <typename T> struct Tanh {
     static Activation<T> init() { return Activation<T>{WK_ACT_TANH}; }
+};
+template <typename T> struct Identity {
+    static Activation<T> init() { return Activation<T>{IDENTITY}; }
 };
 
 // ---- Layer interface (src/nn/layer/main.zig: the vtable) ---------------------------------------
@@ -114,6 +126,7 @@ template <typename T> struct Layer {
     virtual void backward(Pipeline *pipeline, void *cache, TensorT *input, TensorT *input_gradient) const = 0;
     virtual std::vector<TensorT *> getGradients(const void *cache) const = 0;
     virtual std::vector<TensorT *> getBiasGradients(const void *cache) const = 0; // entries may be null
+    virtual void setTraining(bool) {} // no counterpart in the reference: what Dropout listens to
 };
 
 // ---- Linear ------------------------------------------------------------------------------------
@@ -229,7 +242,7 @@ template <typename T> struct Linear : Layer<T> {
                                           input->cols(), input->buffer, input->memory_layout.row_pitch, weights[i]->buffer,
                                           weights[i]->memory_layout.row_pitch, out->buffer, out->memory_layout.row_pitch,
                                           bias_enabled ? bias[i]->buffer : nullptr,
-                                          activation ? activation->kind : WK_ACT_NONE));
+                                          activation && activation->kind != IDENTITY ? activation->kind : WK_ACT_NONE));
             pipeline->append(1);
             input = out;
         }
@@ -252,10 +265,16 @@ template <typename T> struct Linear : Layer<T> {
             TensorT *dev = c->acti_derivatives[i];
             helpers::eqlTensorsShape<T>(sens, dev);
             helpers::eqlTensorsShape<T>(sens, c->outputs[i]);
-            check(wk_sensitivity_step(pipeline->command_queue->stream, core::getTypeIndex<T>(),
-                                      activation ? activation->kind : WK_ACT_NONE, sens->rows(), sens->cols(), c->outputs[i]->buffer,
-                                      c->outputs[i]->memory_layout.row_pitch, sens->buffer, sens->memory_layout.row_pitch, dev->buffer,
-                                      dev->memory_layout.row_pitch, bias_enabled ? c->bias_gradients[i]->buffer : nullptr));
+            if (activation && activation->kind == IDENTITY) {
+                if (bias_enabled) // the sensitivity stays what it is
+                    check(wk_bias_step(pipeline->command_queue->stream, core::getTypeIndex<T>(), sens->rows(), sens->cols(), sens->buffer,
+                                       sens->memory_layout.row_pitch, c->bias_gradients[i]->buffer));
+            } else {
+                check(wk_sensitivity_step(pipeline->command_queue->stream, core::getTypeIndex<T>(),
+                                          activation ? activation->kind : WK_ACT_NONE, sens->rows(), sens->cols(), c->outputs[i]->buffer,
+                                          c->outputs[i]->memory_layout.row_pitch, sens->buffer, sens->memory_layout.row_pitch, dev->buffer,
+                                          dev->memory_layout.row_pitch, bias_enabled ? c->bias_gradients[i]->buffer : nullptr));
+            }
             pipeline->append(1);
             // weight gradient: sens^T [O,B] * prev_output [B,I]
             blas::gemm<T>(pipeline, std::nullopt, sens, blas::Operation::transpose, prev_output, blas::Operation::no_transpose,
@@ -277,6 +296,71 @@ template <typename T> struct Linear : Layer<T> {
     }
 };
 
+// ---- Dropout -----------------------------------------------------------------------------------
+// No counterpart in the reference.  random::dropout between two layers, `width` columns: every forward pass takes the layer's
+// next count, which its cache keeps for the backward pass.  setTraining(false): the outputs are the inputs.
+template <typename T> struct Dropout : Layer<T> {
+    using TensorT = Tensor<T>;
+    struct DropoutCache {
+        TensorT *output = nullptr, *sensitivity = nullptr;
+        uint64_t count = 0; // of the last forward pass
+        double p = 0.0;     // what it dropped
+    };
+    const Context *context = nullptr;
+    uint64_t width = 0, seed = 0;
+    double p = 0.0;
+    bool training = true;
+    mutable std::atomic<uint64_t> count{0};
+
+    static Dropout *init(const Context *context, uint64_t width, double p, std::optional<uint64_t> seed = std::nullopt) {
+        if (!width || !(p >= 0.0 && p <= 1.0)) throw Error(WK_E_INVALID_VALUE);
+        Dropout *d = new Dropout;
+        d->context = context;
+        d->width = width;
+        d->p = p;
+        d->seed = seed ? *seed : (uint64_t)std::chrono::steady_clock::now().time_since_epoch().count();
+        return d;
+    }
+    void setTraining(bool on) override { training = on; }
+    void deinit(Pipeline *) override { delete this; }
+    TensorT *getCachedOutput(const void *cache) const override { return static_cast<const DropoutCache *>(cache)->output; }
+    std::vector<TensorT *> getWeights() const override { return {}; }
+    std::vector<TensorT *> getBias() const override { return {}; }
+    void *prepareCache(Pipeline *pipeline, uint64_t number_of_elements) const override {
+        if (number_of_elements == 0) throw Error(WK_E_INVALID_VALUE);
+        auto c = std::make_unique<DropoutCache>();
+        try {
+            c->output = TensorT::alloc(context, pipeline, {number_of_elements, width});
+            c->sensitivity = TensorT::alloc(context, pipeline, {number_of_elements, width});
+            fill::one<T>(pipeline, c->sensitivity);
+        } catch (...) {
+            releaseCache(pipeline, c.release());
+            throw;
+        }
+        return c.release();
+    }
+    void releaseCache(Pipeline *pipeline, void *cache) const override {
+        DropoutCache *c = static_cast<DropoutCache *>(cache);
+        if (c->output) c->output->release(pipeline);
+        if (c->sensitivity) c->sensitivity->release(pipeline);
+        delete c;
+    }
+    TensorT *forward(Pipeline *pipeline, TensorT *input, void *cache) const override {
+        DropoutCache *c = static_cast<DropoutCache *>(cache);
+        c->p = training ? p : 0.0;
+        c->count = training ? count.fetch_add(1) : 0;
+        random::dropout<T>(pipeline, input, c->output, c->p, seed, c->count);
+        return c->output;
+    }
+    TensorT *getSensitivity(const void *cache) const override { return static_cast<const DropoutCache *>(cache)->sensitivity; }
+    void backward(Pipeline *pipeline, void *cache, TensorT *, TensorT *input_sensitivity) const override {
+        DropoutCache *c = static_cast<DropoutCache *>(cache);
+        if (input_sensitivity) random::dropout<T>(pipeline, c->sensitivity, input_sensitivity, c->p, seed, c->count);
+    }
+    std::vector<TensorT *> getGradients(const void *) const override { return {}; }
+    std::vector<TensorT *> getBiasGradients(const void *) const override { return {}; }
+};
+
 // ---- Sequential --------------------------------------------------------------------------------
 template <typename T> struct Sequential : Layer<T> {
     using TensorT = Tensor<T>;
@@ -288,6 +372,9 @@ template <typename T> struct Sequential : Layer<T> {
     // Sequential.init / append (sequential.zig:40-90): starts empty, owns what is appended
     static Sequential *init() { return new Sequential; }
     void append(Layer<T> *layer) { layers.push_back(layer); }
+    void setTraining(bool on) override {
+        for (Layer<T> *l : layers) l->setTraining(on);
+    }
     void deinit(Pipeline *pipeline) override {
         for (Layer<T> *l : layers) l->deinit(pipeline);
         delete this;
@@ -392,8 +479,101 @@ template <typename T> struct Cache {
     }
 };
 
+// ---- log probabilities of tokens (no counterpart in the reference) --------------------------------------
+// Results and workspace of wk_token_logprobs for {rows, vocab} logits: for scoring and serving (with the `top` likeliest
+// tokens) and for training.  T: f32, f64, F16, BF16; results are f32 (f64 for f64).
+template <typename T> struct TokenLogProbs {
+    using S = std::conditional_t<std::is_same_v<T, double>, double, float>;
+    uint64_t rows = 0, vocab = 0;
+    uint32_t top = 0;
+    Tensor<S> *logprob = nullptr, *lse = nullptr, *entropy = nullptr; // {rows}
+    Tensor<int32_t> *top_ids = nullptr;                               // {rows * top}, row by row; null without alternatives
+    Tensor<S> *top_logprobs = nullptr;
+    Tensor<S> *minus_one = nullptr; // {rows}: the gradient of a loss that is the sum of -logprob
+    wk_device *device = nullptr;
+    void *workspace = nullptr;
+    size_t workspace_bytes = 0;
+
+    static TokenLogProbs *init(const Context *context, Pipeline *pipeline, uint64_t rows, uint64_t vocab, uint32_t top = 0) {
+        if (!rows || !vocab || top > WK_TOKEN_TOP_MAX || top > vocab) throw Error(WK_E_INVALID_VALUE);
+        TokenLogProbs *t = new TokenLogProbs;
+        t->rows = rows;
+        t->vocab = vocab;
+        t->top = top;
+        t->device = context->device;
+        try {
+            for (Tensor<S> **r : {&t->logprob, &t->lse, &t->entropy, &t->minus_one}) *r = Tensor<S>::alloc(context, pipeline, {rows});
+            fill::constant<S>(pipeline, t->minus_one, S(-1));
+            if (top) {
+                t->top_ids = Tensor<int32_t>::alloc(context, pipeline, {rows * top});
+                t->top_logprobs = Tensor<S>::alloc(context, pipeline, {rows * top});
+            }
+            t->workspace_bytes = wk_token_logprobs_workspace_bytes(core::getTypeIndex<T>(), rows, vocab, top);
+            if (t->workspace_bytes) check(wk_malloc(t->device, t->workspace_bytes, &t->workspace));
+        } catch (...) {
+            t->deinit(pipeline);
+            throw;
+        }
+        return t;
+    }
+    void deinit(Pipeline *pipeline) {
+        pipeline->waitAndCleanup();
+        for (Tensor<S> *r : {logprob, lse, entropy, minus_one, top_logprobs})
+            if (r) r->release(pipeline);
+        if (top_ids) top_ids->release(pipeline);
+        if (workspace) wk_free(device, workspace);
+        delete this;
+    }
+    template <typename Id> void validate(const Tensor<T> *logits, const Tensor<Id> *targets) const {
+        static_assert(std::is_same_v<Id, int32_t> || std::is_same_v<Id, int64_t>);
+        if (logits->context != lse->context || (targets && targets->context != lse->context)) throw Error(WK_E_UNQUAL_TENSORS_CONTEXT);
+        if (logits->depth() != 1 || logits->rows() != rows || logits->cols() != vocab) throw Error(WK_E_UNQUAL_TENSORS_SHAPE);
+        if (targets && targets->dimensions.shape != std::vector<uint64_t>{rows}) throw Error(WK_E_UNQUAL_TENSORS_SHAPE);
+    }
+    // targets null: no logprob
+    template <typename Id> void forward(Pipeline *pipeline, const Tensor<T> *logits, const Tensor<Id> *targets) {
+        validate(logits, targets);
+        check(wk_token_logprobs(pipeline->command_queue->stream, core::getTypeIndex<T>(), rows, vocab, logits->buffer,
+                                logits->memory_layout.row_pitch, targets ? targets->buffer : nullptr, core::getTypeIndex<Id>(),
+                                targets ? logprob->buffer : nullptr, lse->buffer, entropy->buffer, top,
+                                top ? static_cast<int32_t *>(top_ids->buffer) : nullptr, top ? top_logprobs->buffer : nullptr, workspace,
+                                workspace_bytes));
+        pipeline->append(1);
+    }
+    // after forward on the same logits; logits_grad may be logits; logprob_grad, entropy_grad {rows}, either null
+    template <typename Id>
+    void backward(Pipeline *pipeline, const Tensor<T> *logits, const Tensor<Id> *targets, const Tensor<S> *logprob_grad,
+                  const Tensor<S> *entropy_grad, Tensor<T> *logits_grad) {
+        validate(logits, targets);
+        helpers::eqlTensorsShape<T>(logits, logits_grad);
+        for (const Tensor<S> *g : {logprob_grad, entropy_grad})
+            if (g && g->dimensions.shape != std::vector<uint64_t>{rows}) throw Error(WK_E_UNQUAL_TENSORS_SHAPE);
+        check(wk_token_logprobs_grad(pipeline->command_queue->stream, core::getTypeIndex<T>(), rows, vocab, logits->buffer,
+                                     logits->memory_layout.row_pitch, targets ? targets->buffer : nullptr, core::getTypeIndex<Id>(), lse->buffer,
+                                     entropy->buffer, logprob_grad ? logprob_grad->buffer : nullptr,
+                                     entropy_grad ? entropy_grad->buffer : nullptr, logits_grad->buffer, logits_grad->memory_layout.row_pitch));
+        pipeline->append(1);
+    }
+};
+
 // ---- loss ------------------------------------------------------------------------------------------
 namespace loss {
+// No counterpart in the reference: the loss of a network whose outputs are logits over a vocabulary, minus the log probability
+// of each row's target.  As mse does, the derivative goes into the last layer's sensitivity without a factor 1 / rows; error_result,
+// when wanted, is the mean over all rows (this synchronises the pipeline).  A negative target counts nothing and has no gradient.
+template <typename T, typename Id>
+void tokens(bool calculate_derivative, Pipeline *pipeline, Tensor<T> *output, Tensor<Id> *targets, TokenLogProbs<T> *state,
+            const Cache<T> *cache, T *error_result) {
+    if (!targets) throw Error(WK_E_INVALID_VALUE);
+    const auto &last = cache->slots.back();
+    Tensor<T> *sens = last.layer->getSensitivity(last.cache);
+    helpers::eqlTensorsShape<T>(output, sens);
+    state->forward(pipeline, output, targets);
+    if (calculate_derivative)
+        state->template backward<Id>(pipeline, output, targets, state->minus_one, nullptr, sens);
+    if (error_result) *error_result = -math::mean<T>(pipeline, state->logprob);
+}
+
 // mse (src/nn/loss/mse.zig:63-132): error_tensor = (expected - output)^2; with calculate_derivative
 // the last layer's sensitivity receives -2 (expected - output); error_result, when wanted, is the
 // mean of error_tensor (this synchronises the pipeline, as math.mean does).

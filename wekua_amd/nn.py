@@ -34,6 +34,7 @@ class ActivationKind(enum.IntEnum):
     none = -1
     sigmoid = 0
     tanh = 1
+    identity = 2
 
 
 class Activation:
@@ -60,6 +61,15 @@ class Tanh:
     @staticmethod
     def init() -> Activation:
         return Activation(ActivationKind.tanh)
+
+
+class Identity:
+    """The activation of a last layer whose outputs are logits: the derivative is one (the reference's layers without
+    an activation get zero gradients)."""
+
+    @staticmethod
+    def init() -> Activation:
+        return Activation(ActivationKind.identity)
 
 
 class Layer:
@@ -104,6 +114,10 @@ class Layer:
     def getSensitivity(self, layer_cache):
         return self._tensors(5, layer_cache)[0]
 
+    def setTraining(self, on: bool) -> None:
+        """Of a Dropout, or of the Dropout layers in a Sequential: off, their outputs are their inputs."""
+        _w._check(_w._lib().wkz_nn_layer_set_training(self._h, int(on)), "Layer.setTraining")
+
     def forward(self, pipeline, input_tensor, layer_cache):
         h = vp()
         _w._check(_w._lib().wkz_nn_layer_forward(self._h, pipeline._h, input_tensor._h, layer_cache, ctypes.byref(h)),
@@ -127,6 +141,18 @@ class Linear(Layer):
         _w._check(_w._lib().wkz_nn_linear_init(context._h, pipeline._h, dtype_id(dtype), input, output,
                                                int(acti.kind) if acti is not None else -1, deep, int(enable_bias),
                                                seed_arg, ctypes.byref(h)), "Linear.init")
+        return cls(h, dtype, context)
+
+
+class Dropout(Layer):
+    """random.dropout as a layer of `width` columns; every forward pass draws the next mask.  No counterpart in the
+    reference."""
+
+    @classmethod
+    def init(cls, dtype: str, context, width: int, p: float, seed: "int | None" = None) -> "Dropout":
+        h = vp()
+        seed_arg = ctypes.byref(u64(seed)) if seed is not None else None
+        _w._check(_w._lib().wkz_nn_dropout_init(context._h, dtype_id(dtype), width, float(p), seed_arg, ctypes.byref(h)), "Dropout.init")
         return cls(h, dtype, context)
 
 
@@ -180,7 +206,65 @@ class Cache:
             self._h = None
 
 
+class TokenLogProbs:
+    """Log probabilities of given tokens over {rows, vocab} logits with entropy and the `top` likeliest tokens, and their
+    gradient.  dtype (of the logits): f32, f64, f16, bf16; results are f32 (f64 for f64).  No counterpart in the reference."""
+
+    def __init__(self, handle, dtype: str, context, rows: int, top: int):
+        self._h = handle
+        self.dtype, self.context, self.rows, self.top = dtype, context, rows, top
+
+    @classmethod
+    def init(cls, dtype: str, context, pipeline, rows: int, vocab: int, top: int = 0) -> "TokenLogProbs":
+        h = vp()
+        _w._check(_w._lib().wkz_nn_token_logprobs_init(context._h, pipeline._h, dtype_id(dtype), rows, vocab, top, ctypes.byref(h)),
+                  "TokenLogProbs.init")
+        return cls(h, dtype, context, rows, top)
+
+    def deinit(self, pipeline) -> None:
+        if self._h:
+            _w._check(_w._lib().wkz_nn_token_logprobs_deinit(self._h, pipeline._h), "TokenLogProbs.deinit")
+            self._h = None
+
+    def _tensor(self, which: int):
+        h = vp()
+        _w._check(_w._lib().wkz_nn_token_logprobs_tensor(self._h, which, ctypes.byref(h)), "TokenLogProbs")
+        return _w.Tensor._borrow(h, "i32" if which == 3 else "f64" if self.dtype == "f64" else "f32", self.context) if h else None
+
+    logprob = property(lambda self: self._tensor(0))
+    lse = property(lambda self: self._tensor(1))
+    entropy = property(lambda self: self._tensor(2))
+    top_ids = property(lambda self: self._tensor(3), doc="{rows * top}, row by row, or None")
+    top_logprobs = property(lambda self: self._tensor(4))
+
+    def forward(self, pipeline, logits, targets=None) -> None:
+        """targets: an i32 or i64 tensor {rows}; None: no log probabilities, the rest all the same."""
+        _w._check(_w._lib().wkz_nn_token_logprobs_forward(self._h, pipeline._h, logits._h, targets._h if targets is not None else None),
+                  "TokenLogProbs.forward")
+
+    def backward(self, pipeline, logits, targets, logprob_grad, entropy_grad, logits_grad) -> None:
+        """After forward on the same logits; either gradient {rows} may be None; logits_grad may be logits."""
+        def h(t):
+            return t._h if t is not None else None
+        _w._check(_w._lib().wkz_nn_token_logprobs_backward(self._h, pipeline._h, logits._h, h(targets), h(logprob_grad), h(entropy_grad),
+                                                           logits_grad._h), "TokenLogProbs.backward")
+
+
 class loss:
+    @staticmethod
+    def tokens(calculate_derivative: bool, pipeline, output, targets, state: TokenLogProbs, cache: Cache,
+               error_result: "np.ndarray | None"):
+        """Minus the log probability of each row's target token.  The derivative goes into the last layer's sensitivity without
+        a factor 1 / rows, as mse does; `error_result`: a one-element array that receives the mean over all rows (this
+        drains the pipeline), or None.  A negative target counts nothing."""
+        ptr = None
+        if error_result is not None:
+            if error_result.dtype != real_np_dtype(cache.dtype) or error_result.size != 1:
+                raise TypeError("error_result must be a one-element array of the tensors' dtype")
+            ptr = error_result.ctypes.data
+        _w._check(_w._lib().wkz_nn_loss_tokens(int(calculate_derivative), pipeline._h, output._h, targets._h, state._h, cache._h, ptr),
+                  "loss.tokens")
+
     @staticmethod
     def mse(calculate_derivative: bool, pipeline, output, expected, cache: Cache, error_result: "np.ndarray | None"):
         """loss.mse (src/nn/loss/mse.zig:63-132).  `error_result`: a one-element array that receives
