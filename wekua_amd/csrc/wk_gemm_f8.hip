@@ -61,22 +61,20 @@ __device__ __forceinline__ Wide widen_codes(i32x8 c) {
         }
     return w;
 }
+// word i of them
+__device__ __forceinline__ void widen_word(Wide &w, i32x8 c, int i) {
+    const f16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[i], 1.f, false), hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[i], 1.f, true);
+    f16x8 &v = w.v[i / 2];
+    const int at = 4 * (i % 2);
+    v[at] = lo[0];
+    v[at + 1] = lo[1];
+    v[at + 2] = hi[0];
+    v[at + 3] = hi[1];
+}
 __device__ __forceinline__ f32x4 mfma_block(const Wide &rows, const Wide &cols, f32x4 acc) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(rows.v[i], cols.v[i], acc, 0, 0, 0);
     return acc;
-}
-// one block's products of several operands of B with one of A, started in turns
-template <int STEP> __device__ __forceinline__ void start(const i32x8 *rows, i32x8 cols, f32x4 *p) {
-#pragma unroll
-    for (int q = 0; q < STEP; ++q) p[q] = mfma_block(rows[q], cols, f32x4{0.f, 0.f, 0.f, 0.f});
-}
-template <int STEP> __device__ __forceinline__ void start(const Wide *rows, const Wide &cols, f32x4 *p) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int q = 0; q < STEP; ++q)
-            p[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rows[q].v[i], cols.v[i], i ? p[q] : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
 }
 // what a lane's codes become before they are multiplied, by the result's type
 template <typename O> __device__ __forceinline__ auto operand_of(i32x8 c) {
@@ -110,6 +108,22 @@ template <bool ALIGNED> __device__ __forceinline__ i32x4 load_chunk(const uint8_
     return v;
 }
 
+// Sigmoid and tanh of a sum from one exponential of a negative number, without branches, to 2^-21 of the value:
+//   e = exp(-c |x|), r = 1 / (1 + e);  c = 1: sigmoid = r (x >= 0) or e r;  c = 2: tanh = +-(1 - e) r, and below 1/4, where that
+//   difference loses bits, x - x^3/3 + 2 x^5/15 - 17 x^7/315 + 62 x^9/2835 (the next term is below 2^-26 of the sum).
+// (1000 x 4096 x 4096, f32: with the math library's tanh 51.8 us, so 49.0, without an activation 45.0)
+__device__ __forceinline__ float act_of(int kind, float x) {
+    const bool th = kind == WK_ACT_TANH;
+    const float a = __builtin_fabsf(x), c = th ? a + a : a, w = c > 200.f ? 200.f : c; // (not a NaN)
+    const float t = w * 1.44269502f, d = __builtin_fmaf(w, 1.44269502f, -t) + w * 1.92596299e-8f; // w log2 e = t + d
+    const float e = __builtin_amdgcn_exp2f(-t) * __builtin_fmaf(d, -0.693147182f, 1.f), r = __builtin_amdgcn_rcpf(1.f + e);
+    if (!th) return x < 0.f ? e * r : r;
+    const float q = x * x;
+    const float series = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(__builtin_fmaf(0.0218694885f, q, -0.0539682540f), q, 0.133333333f), q, -0.333333333f) * q, x, x);
+    return a < 0.25f ? series : __builtin_copysignf((1.f - e) * r, x);
+}
+
+
 template <typename O, bool ACT = true> __device__ __forceinline__ void store_row4(const F8Args &a, uint32_t m, uint32_t n, f32x4 v) {
     if (m >= a.M || n >= a.N) return;
     O *p = static_cast<O *>(a.C) + (uint64_t)m * a.ldc + n;
@@ -119,7 +133,7 @@ template <typename O, bool ACT = true> __device__ __forceinline__ void store_row
     for (int e = 0; e < 4; ++e) {
         float y = v[e];
         if (a.bias) y += a.bias[whole || n + e < a.N ? n + e : n];
-        out[e] = (O)(ACT ? act_forward<float>(a.kind, y) : y);
+        out[e] = (O)(ACT && a.kind != WK_ACT_NONE ? act_of(a.kind, y) : y);
     }
     if (whole) {
         __builtin_memcpy(p, out, sizeof out);
@@ -133,7 +147,7 @@ template <typename O, bool ACT = true> __device__ __forceinline__ void store_row
 // 128 x 128 tile of C, four wavefronts with 64 x 64 each; k-blocks go through registers into LDS, the next one's loads in
 // flight while this one's products run.  Rows in LDS are 128 bytes; 16-byte chunk c of row r lies at c ^ (r % 8), so that
 // the eight lanes which LDS serves together read all its banks.
-template <bool ALIGNED, typename O> __global__ __launch_bounds__(256) void gemm_f8_tile_kernel(F8Args a) {
+template <bool ALIGNED, typename O> __global__ __launch_bounds__(256, 2) void gemm_f8_tile_kernel(F8Args a) {
     constexpr int TM = 128, TN = 128;
     __shared__ i32x4 la[TM * 8], lb[TN * 8];
     const uint32_t tiles_m = (a.M + TM - 1) / TM;
@@ -230,33 +244,27 @@ __device__ __forceinline__ void tile_place(uint32_t id, uint32_t tiles, uint32_t
     tm = group * 8 + (rest - tn * rows);
 }
 
-// The direct loads of wk_lds_dma.hpp with five wait states in front: the compiler may form the scalar base in vector registers and
-// read it back (it does, for a block number that hangs on a comparison), a vector instruction that writes a scalar register
-// wants five before a memory instruction reads it, and inside inline assembly nobody else puts them there.
-__device__ __forceinline__ void load16(const void *base, uint32_t byte_offset, uint32_t lds_base) {
-    asm volatile("s_nop 4\n\t"
-                 "global_load_lds_dwordx4 %0, %1"
+// The direct loads of wk_lds_dma.hpp with whole addresses in vector registers.  A scalar base would want five wait states in front, which
+// nobody but this text could put there: the compiler may form it in vector registers and read it back (it does, for a block
+// number that hangs on a comparison), and a vector instruction that writes a scalar register wants them before a memory
+// instruction reads it; eight loads to a block of 2500 cycles paid 160 for them.
+__device__ __forceinline__ void load16(const void *from, uint32_t lds_base) {
+    asm volatile("s_nop 0\n\t"
+                 "global_load_lds_dwordx4 %0, off"
                  :
-                 : "v"(byte_offset), "s"(base), "{m0}"(lds_base)
+                 : "v"(from), "{m0}"(lds_base)
                  : "memory");
 }
-__device__ __forceinline__ void load4(const void *base, uint32_t byte_offset, uint32_t lds_base) {
-    asm volatile("s_nop 4\n\t"
-                 "global_load_lds_dword %0, %1"
+__device__ __forceinline__ void load4(const void *from, uint32_t lds_base) {
+    asm volatile("s_nop 0\n\t"
+                 "global_load_lds_dword %0, off"
                  :
-                 : "v"(byte_offset), "s"(base), "{m0}"(lds_base)
+                 : "v"(from), "{m0}"(lds_base)
                  : "memory");
-}
-// an address that is the same in every lane, where the compiler does not see that it is
-template <typename P> __device__ __forceinline__ const P *same_in_lanes(const P *p) {
-    const uint64_t v = reinterpret_cast<uint64_t>(p);
-    return reinterpret_cast<const P *>((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 |
-                                       (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
 }
 
-// EDGE: some tile of the launch has rows beyond an operand, whose place its last row takes.
 template <typename O, int WM, int WN, int MT, int NT, int STAGES, bool EDGE>
-__global__ __launch_bounds__(WM * WN * 64, 2) void gemm_f8_dma_kernel(F8Args a, uint32_t tiles_m, uint32_t tiles_n) {
+__global__ __launch_bounds__(WM * WN * 64, (WM * WN == 4 && STAGES * (WM * MT + WN * NT) > 36 ? 1 : 2)) void gemm_f8_dma_kernel(F8Args a, uint32_t tiles_m, uint32_t tiles_n) {
     using T = DmaTile<O, WM, WN, MT, NT, STAGES>;
     using namespace lds_dma;
     __shared__ __align__(1024) uint8_t lds[T::LDS];
@@ -274,50 +282,36 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void gemm_f8_dma_kernel(F8Args a, 
     // Loads: instruction q of this wavefront fills the 1 KiB piece q * waves + wave of an operand (eight rows); lane l of it the chunk
     // l % 8 of row l / 8, which is the row's chunk (l % 8) ^ (row % 8).
     constexpr uint32_t WAVES = WM * WN, QA = T::A_BYTES / 1024 / WAVES, QB = T::B_BYTES / 1024 / WAVES;
-    const uint32_t lda = (uint32_t)a.lda, ldb = (uint32_t)a.ldb;
     const uint32_t lrow = wave * 8 + lane / 8, lchunk = ((lane % 8) ^ (lane / 8)) * 16;
     const uint32_t last_a = a.M - 1 - m0, last_b = a.N - 1 - n0;
-    auto row_a = [&](uint32_t q) {
-        const uint32_t r = q * WAVES * 8 + lrow;
-        return (EDGE && r > last_a ? last_a : r) * lda;
-    };
-    auto row_b = [&](uint32_t q) {
-        const uint32_t r = q * WAVES * 8 + lrow;
-        return (EDGE && r > last_b ? last_b : r) * ldb;
-    };
-    const uint32_t off_a = row_a(0) + lchunk, off_b = row_b(0) + lchunk;
+    // (a lane whose row lies behind the edge repeats its first one, the last row if that lies there too)
+    const uint8_t *const from_a = a.A + (m0 + (EDGE && lrow > last_a ? last_a : lrow)) * a.lda + lchunk;
+    const uint8_t *const from_b = a.B + (n0 + (EDGE && lrow > last_b ? last_b : lrow)) * a.ldb + lchunk;
     // In the shorter last block the chunks behind K repeat the last one that has some of it (and are put to zero later).
     const uint32_t rest = a.K % KB, beyond = rest && lchunk > (rest - 1) / 16 * 16 ? lchunk - (rest - 1) / 16 * 16 : 0;
     // Scales: wavefront w brings 64 of A's, rows 64 w ..., in the order in which a lane will want them: place p of 16 MT rows holds row
     // (p % MT) * 16 + p / MT; the wavefronts that are left bring B's, one per 128 columns (all the same ones: a branch here would
     // end the loop's basic block, and what is behind it would be kept waiting)
     const bool for_a = wave * 64 < T::TM;
-    uint32_t off_s;
+    const float *from_s;
     {
         const uint32_t p = wave * 64 + lane, rows = MT * 16, base = p / rows * rows, in = p - base;
         const uint32_t r = base + (in % MT) * 16 + in / MT;
-        off_s = for_a ? (r < last_a ? r : last_a) * (uint32_t)a.sap * 4 : (lane < T::NB && lane * KB <= last_b ? lane : 0) * (uint32_t)a.sbp * 4;
+        from_s = for_a ? a.sa + (m0 + (r < last_a ? r : last_a)) * a.sap : a.sb + (n0 / KB + (lane < T::NB && lane * KB <= last_b ? lane : 0)) * a.sbp;
     }
-    const uint8_t *base_a = a.A + (uint64_t)m0 * a.lda, *base_b = a.B + (uint64_t)n0 * a.ldb;
-    const float *base_s = same_in_lanes(for_a ? a.sa + (uint64_t)m0 * a.sap : a.sb + (uint64_t)(n0 / KB) * a.sbp);
 
-    auto request_scales = [&](uint32_t kb, uint32_t at) {
-        load4(same_in_lanes(base_s + kb), off_s, lds0 + at + T::A_BYTES + T::B_BYTES + wave * 256);
-    };
     constexpr uint32_t PER = QA + QB + 1; // loads of a wavefront per block
     auto request_one = [&](uint32_t kb, uint32_t at, uint32_t n) {
-        const uint32_t to = lds0 + at + wave * 1024, back = kb < whole ? 0 : beyond;
+        const uint32_t to = lds0 + at + wave * 1024;
+        const uint64_t k = (uint64_t)kb * KB - (kb < whole ? 0 : beyond);
         if (n < QA) {
-            const uint8_t *ka = base_a + (uint64_t)kb * KB;
-            if (EDGE && n) load16(ka, row_a(n) + lchunk - back, to + n * WAVES * 1024);
-            else load16(ka + (uint64_t)(n * WAVES * 8) * lda, off_a - back, to + n * WAVES * 1024);
+            const uint32_t r = n * WAVES * 8;
+            load16(from_a + k + (EDGE && n && r + lrow > last_a ? 0 : r * a.lda), to + n * WAVES * 1024);
         } else if (n < QA + QB) {
-            const uint32_t q = n - QA;
-            const uint8_t *kbp = base_b + (uint64_t)kb * KB;
-            if (EDGE && q) load16(kbp, row_b(q) + lchunk - back, to + T::A_BYTES + q * WAVES * 1024);
-            else load16(kbp + (uint64_t)(q * WAVES * 8) * ldb, off_b - back, to + T::A_BYTES + q * WAVES * 1024);
+            const uint32_t q = n - QA, r = q * WAVES * 8;
+            load16(from_b + k + (EDGE && q && r + lrow > last_b ? 0 : r * a.ldb), to + T::A_BYTES + q * WAVES * 1024);
         } else {
-            request_scales(kb, at);
+            load4(from_s + kb, lds0 + at + T::A_BYTES + T::B_BYTES + wave * 256);
         }
     };
     auto request = [&](uint32_t kb, uint32_t at) {
@@ -341,7 +335,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void gemm_f8_dma_kernel(F8Args a, 
     };
 
     f32x4 acc[MT][NT] = {};
-    i32x8 fb[NT], fa[2];
+    i32x8 fb[NT];
     float s[MT], s_b;
     auto read_scales = [&](uint32_t at) {
         const float *p = reinterpret_cast<const float *>(lds + at + T::A_BYTES + T::B_BYTES);
@@ -349,64 +343,147 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void gemm_f8_dma_kernel(F8Args a, 
         for (int i = 0; i < MT; ++i) s[i] = p[wm + r16 * MT + i];
         s_b = p[T::TM + wn / KB];
     };
-    auto first_operands = [&](uint32_t at) {
+    auto meet = [&]() {
+        wait_lgkm0(); // this wavefront has read the block,
+        wait_vm<(STAGES - 2) * PER>(); // and its share of the next one is there
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    // Per block: prepare() its first operands, once; products() of the block at `at`, MORE: on the way the first operands of the next one, at
+    // `next`, and the request of block `ahead`.
+    //
+    // f32 results: the codes of an operand become 16-bit numbers, which takes about as long as its products do, so the two take
+    // turns instruction by instruction.  Under the products of row i: the widening of row i + 1 (behind the last row: of the
+    // next block's first), the scaling of row i - 1 (before the first: of the last block's last), and under the last row's
+    // also the widening of the next block's columns, a quarter at a time as soon as no product wants its predecessor any more.
+    Wide wb[NT], wa[2];
+    f32x4 p[2][NT] = {};
+    float f_last = 0.f; // the scale of the row whose products wait to be added
+    i32x8 raw;
+    auto wide_first = [&](uint32_t at) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) fb[j] = operand(at + at_b + 16 * j * KB);
+        const i32x8 c = operand(at + at_a);
+        raw = operand(at + at_a + 16 * KB);
+        read_scales(at);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) widen_word(wa[0], c, i);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < 6; ++i) widen_word(wb[j], fb[j], i); // (the last quarter: under the first row)
+    };
+    auto add_row = [&](int k, int from, int to, const f32x4 *row, float f) {
+#pragma unroll
+        for (int e = from; e < to; ++e) acc[k][e / 4][e % 4] = __builtin_fmaf(row[e / 4][e % 4], f, acc[k][e / 4][e % 4]);
+    };
+    auto wide_block = [&]<bool MORE>(std::integral_constant<bool, MORE>, uint32_t at, uint32_t next, uint32_t ahead) {
+        static_assert(MT % 2 == 0);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const bool last = i + 1 == MT;
+            const float f = i ? s[(i + MT - 1) % MT] * s_b : f_last;
+            if (last) f_last = s[MT - 1] * s_b;
+            if (last && MORE) read_scales(next);
+#pragma unroll
+            for (int n = 0; n < 4 * NT; ++n) {
+                const int v = n / NT, q = n % NT;
+                p[i & 1][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wb[q].v[v], wa[i & 1].v[v], v ? p[i & 1][q] : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                if (!last || MORE) {
+                    constexpr int EACH = NT < 4 ? 4 / NT : 1; // words of the next row per product, in the first half
+                    if (n < 8 / EACH)
+#pragma unroll
+                        for (int w = 0; w < EACH; ++w) widen_word(wa[(i + 1) & 1], raw, n * EACH + w);
+                }
+                if (i == 0 && n < NT) {
+                    widen_word(wb[n], fb[n], 6);
+                    widen_word(wb[n], fb[n], 7);
+                }
+                if (last && MORE && v) {
+                    widen_word(wb[q], fb[q], 2 * v - 2);
+                    widen_word(wb[q], fb[q], 2 * v - 1);
+                }
+                add_row((i + MT - 1) % MT, n, n + 1, p[(i + 1) & 1], f);
+                if (n == 2 * NT) {
+                    if (i + 2 < MT) {
+                        raw = operand(at + at_a + 16 * (i + 2) * KB);
+                    } else if (MORE) {
+                        if (!last) {
+                            meet();
+#pragma unroll
+                            for (int j = 0; j < NT; ++j) fb[j] = operand(next + at_b + 16 * j * KB);
+                        }
+                        raw = operand(next + at_a + 16 * (i + 2 - MT) * KB);
+                    }
+                }
+                if (last && MORE) { // requests to refill this block's stage
+#pragma unroll
+                    for (uint32_t r = n * PER / (4 * NT); r < (n + 1) * PER / (4 * NT); ++r) request_one(ahead, at, r);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        if (!MORE) {
+            add_row(MT - 1, 0, 4 * NT, p[(MT - 1) & 1], f_last);
+            f_last = 0.f;
+        }
+    };
+    // 16-bit results: a product is one instruction; each is scaled and added three products later.  The order is held as written: a free
+    // schedule lets so many results live at once that registers spill.
+    i32x8 fa[2];
+    auto narrow_first = [&](uint32_t at) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) fb[j] = operand(at + at_b + 16 * j * KB);
         fa[0] = operand(at + at_a);
         read_scales(at);
     };
-    // the products of the block at `at`; MORE: on the way the first operands of the next one, at `next`, and the request of block `ahead`
-    auto block = [&]<bool MORE>(std::integral_constant<bool, MORE>, uint32_t at, uint32_t next, uint32_t ahead) {
-        decltype(operand_of<O>(i32x8{})) wb[NT];
+    auto narrow_block = [&]<bool MORE>(std::integral_constant<bool, MORE>, uint32_t at, uint32_t next, uint32_t ahead) {
+        constexpr int LAG = 3;
+        i32x8 b[NT];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) wb[j] = operand_of<O>(fb[j]);
-        // One step: STEP products of a row are started, those of the step LAG before are scaled and added.  f32: a whole row, whose
-        // four instructions each take turns (each waits for the one before it in its sum).  The order is held as written: a free
-        // schedule lets so many results live at once that registers spill.
-        constexpr bool WIDE = std::is_same_v<O, float>;
-        constexpr int STEP = WIDE ? NT : 1, LAG = WIDE ? 1 : 3, STEPS = MT * NT / STEP;
-        f32x4 p[LAG + 1][STEP];
-        decltype(operand_of<O>(i32x8{})) wa;
+        for (int j = 0; j < NT; ++j) b[j] = fb[j];
+        f32x4 q[LAG + 1];
+        i32x8 row;
 #pragma unroll
-        for (int t = 0; t < STEPS + LAG; ++t) {
-            const int i = t * STEP / NT, j = t * STEP % NT;
-            if (t < STEPS) {
+        for (int t = 0; t < MT * NT + LAG; ++t) {
+            const int i = t / NT, j = t % NT;
+            if (t < MT * NT) {
                 if (j == 0) {
-                    wa = operand_of<O>(fa[i & 1]);
+                    row = fa[i & 1];
                     if (i + 1 < MT) {
                         fa[(i + 1) & 1] = operand(at + at_a + 16 * (i + 1) * KB);
                     } else if (MORE) {
-                        wait_lgkm0(); // this wavefront has read the block,
-                        wait_vm<(STAGES - 2) * PER>(); // and its share of the next one is there
-                        __builtin_amdgcn_s_barrier();
-                        asm volatile("" ::: "memory");
+                        meet();
                     }
                 }
-                start<STEP>(&wb[j], wa, p[t % (LAG + 1)]);
+                q[t % (LAG + 1)] = mfma_block(b[j], row, f32x4{0.f, 0.f, 0.f, 0.f});
                 if (i + 1 == MT && MORE) {
                     // the next block's operands, and requests to refill this one's stage, under the running products
                     __builtin_amdgcn_sched_barrier(0);
                     if (j == 0) fa[(i + 1) & 1] = operand(next + at_a);
+                    fb[j] = operand(next + at_b + 16 * j * KB);
 #pragma unroll
-                    for (int q = j; q < j + STEP; ++q) fb[q] = operand(next + at_b + 16 * q * KB);
-#pragma unroll
-                    for (uint32_t n = j * PER / NT; n < (j + STEP) * PER / NT; ++n) request_one(ahead, at, n);
+                    for (uint32_t n = j * PER / NT; n < (j + 1) * PER / NT; ++n) request_one(ahead, at, n);
                 }
             }
             if (t >= LAG) {
-                const int u = t - LAG, k = u * STEP / NT;
+                const int u = t - LAG, k = u / NT;
                 const float f = s[k] * s_b;
 #pragma unroll
-                for (int q = 0; q < STEP; ++q)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        acc[k][u * STEP % NT + q][e] = __builtin_fmaf(p[u % (LAG + 1)][q][e], f, acc[k][u * STEP % NT + q][e]);
+                for (int e = 0; e < 4; ++e) acc[k][u % NT][e] = __builtin_fmaf(q[u % (LAG + 1)][e], f, acc[k][u % NT][e]);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
         if (MORE) read_scales(next);
     };
-
+    auto prepare = [&](uint32_t at) {
+        if constexpr (std::is_same_v<O, float>) wide_first(at);
+        else narrow_first(at);
+    };
+    auto products = [&](auto more, uint32_t at, uint32_t next, uint32_t ahead) {
+        if constexpr (std::is_same_v<O, float>) wide_block(more, at, next, ahead);
+        else narrow_block(more, at, next, ahead);
+    };
     uint32_t at = 0;
     auto after = [](uint32_t stage) { return stage + T::STAGE == T::LDS ? 0 : stage + T::STAGE; };
     // (requests beyond the last block repeat it, into stages that nobody reads any more: the counts stay the same)
@@ -416,10 +493,10 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void gemm_f8_dma_kernel(F8Args a, 
     if (whole) {
         wait_vm<(STAGES - 1) * PER>();
         __syncthreads();
-        first_operands(0);
+        prepare(0);
         for (uint32_t kb = 0; kb + 1 < whole; ++kb) {
             const uint32_t next = after(at);
-            block(std::true_type{}, at, next, kb + STAGES < last_block ? kb + STAGES : last_block);
+            products(std::true_type{}, at, next, kb + STAGES < last_block ? kb + STAGES : last_block);
             at = next;
         }
     }
@@ -431,9 +508,9 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void gemm_f8_dma_kernel(F8Args a, 
             __syncthreads();
             cut_short(at);
             __syncthreads();
-            first_operands(at);
+            prepare(at);
         }
-        block(std::false_type{}, at, 0, 0);
+        products(std::false_type{}, at, 0, 0);
     }
     wait_vm<0>();
 
@@ -453,7 +530,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void gemm_f8_dma_kernel(F8Args a, 
     for (int first = 0; first < MT * NT; first += PASS) {
 #pragma unroll
         for (int q = 0; q < PASS; ++q) own[q * T::THREADS] = acc[(first + q) / NT][(first + q) % NT];
-#pragma unroll 1
+#pragma unroll 2
         for (int q = 0; q < PASS; ++q)
             store_row4<O, true>(a, m0 + wm + 16 * ((first + q) / NT) + r16, n0 + wn + 16 * ((first + q) % NT) + 4 * g, own[q * T::THREADS]);
     }
@@ -610,18 +687,20 @@ template <typename O> int gemm_f8_launch(wk_stream *s, const F8Args &a, bool ali
     if (a.M <= (direct && !std::is_same_v<O, float> ? 16 : 64)) return aligned ? gemm_f8_rows<true, O>(st, a) : gemm_f8_rows<false, O>(st, a);
     if (direct) {
         if constexpr (std::is_same_v<O, float>) {
-            constexpr TileTime t[] = {{128, 128, 2, 76, 145}, {64, 128, 2, 51, 82}, {64, 64, 2, 35, 48}};
+            constexpr TileTime t[] = {{128, 128, 2, 79, 148}, {64, 128, 2, 50, 85}, {64, 64, 2, 34, 51}};
             switch (best_tile(t, 3, a)) {
             case 0: return gemm_f8_dma_launch<O, 2, 2, 4, 4, 2>(st, a);
             case 1: return gemm_f8_dma_launch<O, 2, 2, 2, 4, 3>(st, a);
             default: return gemm_f8_dma_launch<O, 2, 2, 2, 2, 4>(st, a);
             }
         } else {
-            constexpr TileTime t[] = {{256, 256, 1, 147, 147}, {128, 128, 2, 46, 88}, {64, 128, 2, 29, 51}, {64, 64, 2, 21, 33}};
-            switch (best_tile(t, 4, a)) {
+            // 128 x 128 twice: a third stage for tiles that are alone on their units, two for tiles that share them
+            constexpr TileTime t[] = {{256, 256, 1, 146, 146}, {128, 128, 1, 47, 48}, {128, 128, 2, 57, 86}, {64, 128, 2, 28, 53}, {64, 64, 2, 20, 34}};
+            switch (best_tile(t, 5, a)) {
             case 0: return gemm_f8_dma_launch<O, 2, 4, 8, 4, 2>(st, a);
-            case 1: return gemm_f8_dma_launch<O, 2, 2, 4, 4, 2>(st, a);
-            case 2: return gemm_f8_dma_launch<O, 2, 2, 2, 4, 3>(st, a);
+            case 1: return gemm_f8_dma_launch<O, 2, 2, 4, 4, 3>(st, a);
+            case 2: return gemm_f8_dma_launch<O, 2, 2, 4, 4, 2>(st, a);
+            case 3: return gemm_f8_dma_launch<O, 2, 2, 2, 4, 3>(st, a);
             default: return gemm_f8_dma_launch<O, 2, 2, 2, 2, 4>(st, a);
             }
         }
