@@ -296,7 +296,11 @@ int  wk_to_real(wk_stream *s, int real_dtype, const uint64_t shape3[3], const vo
 
 /* ---- the token end of a network ------------------------------------------------------------------
  * No counterpart in the reference, whose only loss is mse.  Dropout, products of 8-bit floating point with a
- * scale for every block of 128 elements of k, and log probabilities of given tokens with their gradient. */
+ * scale for every block of 128 elements of k, and log probabilities of given tokens with their gradient.
+ * Unless said otherwise a result overlaps no operand.  A launch has fewer than 2^32 threads; a call that would need more answers
+ * WK_E_INVALID_VALUE: dropout takes fewer than 2^34 elements (16-bit types 2^35), the quantiser fewer than 2^31 rows and columns
+ * and, with block_rows 1, 2^35 elements, log probabilities fewer than 2^24 rows (vocab up to 1024: 2^26) and their
+ * gradient fewer than 2^24 rows of up to 2048 tokens (16-bit 4096, f64 1024), of more tokens accordingly fewer. */
 
 /* Dropout: y = x / (1 - p) where an element is kept, 0 where it is dropped (whatever x holds there).  Element i of
  * the logical {depth, rows, cols} region, counted row by row whatever the pitches, is kept when its 32-bit

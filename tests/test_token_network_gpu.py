@@ -632,3 +632,28 @@ def test_more_than_the_cache_holds(dev):
         assert (np.abs(values("bf16", got[r:r + 1]) - want) <= (2.0 ** -8 + 1e-5) * np.abs(want)).all()
     for b in (bx, by, bt, bw, *stats):
         b.free()
+
+
+def test_sizes_beyond_one_launch_are_refused(dev):
+    """More threads than a launch counts, results in an operand's place: refused on the host."""
+    b = dev.malloc(1 << 12)
+    p, lib, st = b.ptr.value, dev.lib, dev.stream
+    q = p + 2048
+    s3 = ctypes.c_uint64 * 3
+    for dtype, per in ((8, 4), (9, 4), (32, 8), (33, 8)):
+        n = per * 2 ** 32
+        assert lib.wk_dropout(st, dtype, s3(1, 1, n), p, n, n, p, n, n, 0.5, 1, 0, None) == 1
+        assert lib.wk_dropout(st, dtype, s3(2 ** 16, 2 ** 16, 1), p, 1, 2 ** 16, q, 2, 2 ** 17, 0.5, 1, 0, None) == 1
+    for rows, cols in ((2 ** 28, 128), (1, 2 ** 31), (2 ** 31, 1), (2 ** 40 - 1, 2 ** 40 - 1)):
+        assert lib.wk_f8_quantize(st, 33, rows, cols, p, cols, 1, q, cols, p + 1024, -(-cols // 128)) == 1
+    assert lib.wk_f8_quantize(st, 33, 2 ** 30, 2 ** 29, p, 2 ** 29, 128, q, 2 ** 29, p + 1024, 2 ** 22) == 1
+    assert lib.wk_f8_quantize(st, 33, 2, 8, p, 8, 1, p, 8, q, 1) == 1
+    assert lib.wk_gemm_f8(st, 1, 2 ** 31 - 1, 16, p, 16, p, 1, q, 16, p, 1, 8, p + 1024, 2 ** 31, None, -1) == 1
+    assert lib.wk_gemm_f8(st, 2 ** 30, 2 ** 30, 16, p, 16, p, 1, q, 16, p, 1, 8, p + 1024, 2 ** 31, None, -1) == 1
+    for c in (p, q):
+        assert lib.wk_gemm_f8(st, 2, 2, 16, p, 16, p + 512, 1, q, 16, p + 512, 1, 8, c, 2, None, -1) == 1
+    for rows, vocab in ((2 ** 24, 1025), (2 ** 26, 1024), (2 ** 31, 1), (2, 2 ** 31)):
+        assert lib.wk_token_logprobs(st, 8, rows, vocab, p, vocab, None, 4, None, q, None, 0, None, None, None, 0) == 1
+    for dtype, rows, vocab in ((8, 2 ** 24, 1), (8, 2 ** 23, 2049), (33, 2 ** 23, 4097), (9, 2 ** 23, 1025)):
+        assert lib.wk_token_logprobs_grad(st, dtype, rows, vocab, p, vocab, q, 4, q, None, q, None, p, vocab) == 1
+    b.free()

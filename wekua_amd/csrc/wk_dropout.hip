@@ -135,7 +135,7 @@ template <typename T> int dropout_launch(wk_stream *s, const void *x, void *y, D
     }
     const W scale = p < 1.0 ? (W)(1.0 / (1.0 - p)) : W(0);
     const uint64_t per_row = (a.cols + PER - 1) / PER, chunks = per_row * a.total_rows;
-    if ((chunks + 255) / 256 > 0x7fffffffull) return WK_E_INVALID_VALUE;
+    if ((chunks + 255) / 256 > most_groups(256)) return WK_E_INVALID_VALUE;
     const bool phase0 = a.total_rows == 1 || a.cols % 4 == 0, stream = 2 * a.total_rows * a.cols * sizeof(T) > (256ull << 20);
     if (phase0) (stream ? dropout_enqueue<T, PER, true, true> : dropout_enqueue<T, PER, true, false>)(s->stream, chunks, per_row, x, y, a, scale);
     else (stream ? dropout_enqueue<T, PER, false, true> : dropout_enqueue<T, PER, false, false>)(s->stream, chunks, per_row, x, y, a, scale);

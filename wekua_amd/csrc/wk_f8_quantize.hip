@@ -134,7 +134,7 @@ int quantize_launch(wk_stream *s, uint64_t rows, uint64_t cols, const void *x, u
                     uint64_t q_pitch, float *scales, uint64_t scale_pitch) {
     const uint64_t col_blocks = (cols + KB - 1) / KB;
     const uint64_t groups = block_rows == 1 ? (rows * col_blocks + 256 / LANES - 1) / (256 / LANES) : (rows + KB - 1) / KB * col_blocks;
-    if (groups > 0x7fffffffull) return WK_E_INVALID_VALUE;
+    if (groups > most_groups(256)) return WK_E_INVALID_VALUE;
     if (block_rows == 1)
         hipLaunchKernelGGL(quantize_rows_kernel<T>, dim3((unsigned)groups), dim3(256), 0, s->stream, static_cast<const T *>(x), pitch, rows,
                            cols, static_cast<uint8_t *>(q), q_pitch, scales, scale_pitch, col_blocks);
@@ -154,7 +154,7 @@ extern "C" int wk_f8_quantize(wk_stream *s, int dtype, uint64_t rows, uint64_t c
     int rc = bind(s);
     if (rc) return rc;
     if (!rows || !cols || !x || !q || !scales || (block_rows != 1 && block_rows != KB)) return WK_E_INVALID_VALUE;
-    if (rows >> 40 || cols >> 40) return WK_E_INVALID_VALUE;
+    if (rows >> 31 || cols >> 31 || q == x) return WK_E_INVALID_VALUE;
     const uint64_t scale_rows = (rows + block_rows - 1) / block_rows;
     if (rows > 1 && (pitch < cols || q_pitch < cols)) return WK_E_INVALID_VALUE;
     if (scale_rows > 1 && scale_pitch < (cols + KB - 1) / KB) return WK_E_INVALID_VALUE;

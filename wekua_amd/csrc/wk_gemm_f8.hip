@@ -539,7 +539,7 @@ __global__ __launch_bounds__(WM * WN * 64, (WM * WN == 4 && STAGES * (WM * MT + 
 template <typename O, int WM, int WN, int MT, int NT, int STAGES> int gemm_f8_dma_launch(hipStream_t st, const F8Args &a) {
     using T = DmaTile<O, WM, WN, MT, NT, STAGES>;
     const uint64_t tiles_m = (a.M + T::TM - 1) / T::TM, tiles_n = (a.N + T::TN - 1) / T::TN;
-    if (tiles_m * tiles_n > 0x7fffffffull) return WK_E_INVALID_VALUE;
+    if (tiles_m * tiles_n > most_groups(T::THREADS)) return WK_E_INVALID_VALUE;
     const dim3 grid((unsigned)(tiles_m * tiles_n)), block(T::THREADS);
     if (a.M % T::TM || a.N % T::TN)
         hipLaunchKernelGGL((gemm_f8_dma_kernel<O, WM, WN, MT, NT, STAGES, true>), grid, block, 0, st, a, (uint32_t)tiles_m, (uint32_t)tiles_n);
@@ -641,8 +641,9 @@ template <bool ALIGNED, typename O, int MT, int NT, int DEEP, uint32_t WAVES = 8
 }
 
 template <bool ALIGNED, typename O, int MT, int NT, int DEEP, uint32_t WAVES = 8> int gemm_f8_rows_launch(hipStream_t st, const F8Args &a) {
-    hipLaunchKernelGGL((gemm_f8_rows_kernel<ALIGNED, O, MT, NT, DEEP, WAVES>), dim3((a.N + 16 * NT - 1) / (16 * NT), (a.M + 16 * MT - 1) / (16 * MT)),
-                       dim3(WAVES * 64), 0, st, a);
+    const uint32_t across = (a.N + 16 * NT - 1) / (16 * NT);
+    if (across > most_groups(WAVES * 64)) return WK_E_INVALID_VALUE;
+    hipLaunchKernelGGL((gemm_f8_rows_kernel<ALIGNED, O, MT, NT, DEEP, WAVES>), dim3(across, (a.M + 16 * MT - 1) / (16 * MT)), dim3(WAVES * 64), 0, st, a);
     return launch_status();
 }
 
@@ -706,7 +707,7 @@ template <typename O> int gemm_f8_launch(wk_stream *s, const F8Args &a, bool ali
         }
     }
     const uint64_t tiles = (uint64_t)((a.M + 127) / 128) * ((a.N + 127) / 128);
-    if (tiles > 0x7fffffffull) return WK_E_INVALID_VALUE;
+    if (tiles > most_groups(256)) return WK_E_INVALID_VALUE;
     if (aligned)
         hipLaunchKernelGGL((gemm_f8_tile_kernel<true, O>), dim3((unsigned)tiles), dim3(256), 0, st, a);
     else
@@ -722,7 +723,7 @@ extern "C" int wk_gemm_f8(wk_stream *s, uint64_t M, uint64_t N, uint64_t K, cons
     int rc = bind(s);
     if (rc) return rc;
     if (!M || !N || !K || !A || !B || !C || !a_scales || !b_scales) return WK_E_INVALID_VALUE;
-    if (M >> 31 || N >> 31 || K >> 31) return WK_E_INVALID_VALUE;
+    if (M >> 31 || N >> 31 || K >> 31 || C == A || C == B) return WK_E_INVALID_VALUE;
     const uint64_t kblocks = (K + KB - 1) / KB;
     if (lda < K || ldb < K || ldc < N || a_scale_pitch < kblocks || b_scale_pitch < kblocks) return WK_E_INVALID_VALUE;
     if (kind != WK_ACT_NONE && kind != WK_ACT_SIGMOID && kind != WK_ACT_TANH) return WK_E_INVALID_VALUE;

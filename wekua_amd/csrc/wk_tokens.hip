@@ -489,7 +489,7 @@ int logprobs_launch(wk_stream *s, uint64_t rows, uint32_t vocab, const void *log
     A *ws = static_cast<A *>(workspace);
     int32_t *ids = parts > 1 ? reinterpret_cast<int32_t *>(ws + (size_t)rows * parts * (3 + top)) : nullptr;
     const uint64_t units = rows * parts;
-    if (units > 0x7fffffffull) return WK_E_INVALID_VALUE;
+    if ((parts == 1 && vocab <= 1024 ? (units + 3) / 4 : units) > most_groups(256)) return WK_E_INVALID_VALUE;
     if (parts == 1 && vocab <= 1024) logprobs_enqueue<T, 1>(s->stream, (unsigned)((units + 3) / 4), x, pitch, rows, vocab, part_len, parts, top, o, ws, ids);
     else logprobs_enqueue<T, 4>(s->stream, (unsigned)units, x, pitch, rows, vocab, part_len, parts, top, o, ws, ids);
     if (parts > 1) {
@@ -587,7 +587,7 @@ int grad_launch(wk_stream *s, uint64_t rows, uint32_t vocab, const void *x, uint
                 const GradArgs<typename stat_of<T>::type> &a) {
     constexpr uint32_t step = 256 * GRAD_DEEP * 16 / sizeof(T);
     const uint32_t segments = (vocab + step - 1) / step;
-    if (rows * segments > 0x7fffffffull) return WK_E_INVALID_VALUE;
+    if (rows * segments > most_groups(256)) return WK_E_INVALID_VALUE;
     const bool stream = 2 * rows * vocab * sizeof(T) > (256ull << 20);
     if (a.h) (stream ? grad_enqueue<T, true, true> : grad_enqueue<T, true, false>)(s->stream, rows, vocab, x, pitch, dx, grad_pitch, segments, a);
     else (stream ? grad_enqueue<T, false, true> : grad_enqueue<T, false, false>)(s->stream, rows, vocab, x, pitch, dx, grad_pitch, segments, a);
