@@ -70,9 +70,14 @@ __device__ __forceinline__ void store8(uint8_t *p, uint64_t left, const float v[
     }
 }
 
+// STREAM, here and below: the last-level cache (256 MB) would not hold x and what comes next, so x passes it by, and what lies there
+// unwritten need not be put out for it.  Measured (8192 x 8192, us) with a cache full of other writes, then without: per block
+// f32 90 -> 65 and 62 -> 61, bf16 64 -> 42 and 37 -> 37; 4096 x 4096 f32, which it holds, 15 -> 19.  The codes stay in
+// the cache for the product: past it, another 5 us less here were 13 more there.
+//
 // One scale per row and 128 columns: sixteen lanes to a block, sixteen blocks to a work-group.  Bound by memory: 8192 x 8192 f32
-// 58 us (5.8 TB/s), bf16 41.
-template <typename T>
+// 60 us (5.6 TB/s), bf16 38.
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T *__restrict__ x, uint64_t pitch, uint64_t rows, uint64_t cols,
                                                             uint8_t *__restrict__ q, uint64_t q_pitch, float *__restrict__ scales,
                                                             uint64_t scale_pitch, uint64_t col_blocks) {
@@ -82,7 +87,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T *__restrict_
     const uint64_t row = in ? blk / col_blocks : 0, cb = in ? blk - row * col_blocks : 0;
     const uint64_t c = cb * KB + lane * PER, left = in && c < cols ? cols - c : 0;
     float v[PER], amax = 0.f;
-    load8<false>(x + row * pitch + (left ? c : 0), left, v);
+    load8<STREAM>(x + row * pitch + (left ? c : 0), left, v);
 #pragma unroll
     for (int e = 0; e < PER; ++e) amax = larger(amax, __builtin_fabsf(v[e]));
 #pragma unroll
@@ -94,9 +99,8 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T *__restrict_
 }
 
 // One scale per 128 x 128 block: a work-group holds the block in registers, 8 columns of every 16th row to a thread.  Bound by
-// memory: 8192 x 8192 f32 58 us (5.8 TB/s), bf16 36.  STREAM: the last-level cache (256 MB) would not hold x and what
-// comes next, so x passes it by (bf16 44 -> 36 us; 4096 x 4096 f32, which it holds, 15 -> 19).  Four blocks side by side
-// to a work-group of 1024 threads, for longer runs of memory, were slower (74 us).
+// memory: 8192 x 8192 f32 60 us (5.6 TB/s), bf16 37.  Four blocks side by side to a work-group of 1024 threads, for longer runs of
+// memory, were slower (74 us), runs of eight blocks to a die no faster (61).
 template <typename T, bool STREAM>
 __global__ __launch_bounds__(256) void quantize_blocks_kernel(const T *__restrict__ x, uint64_t pitch, uint64_t rows, uint64_t cols,
                                                               uint8_t *__restrict__ q, uint64_t q_pitch, float *__restrict__ scales,
@@ -135,15 +139,11 @@ int quantize_launch(wk_stream *s, uint64_t rows, uint64_t cols, const void *x, u
     const uint64_t col_blocks = (cols + KB - 1) / KB;
     const uint64_t groups = block_rows == 1 ? (rows * col_blocks + 256 / LANES - 1) / (256 / LANES) : (rows + KB - 1) / KB * col_blocks;
     if (groups > most_groups(256)) return WK_E_INVALID_VALUE;
-    if (block_rows == 1)
-        hipLaunchKernelGGL(quantize_rows_kernel<T>, dim3((unsigned)groups), dim3(256), 0, s->stream, static_cast<const T *>(x), pitch, rows,
-                           cols, static_cast<uint8_t *>(q), q_pitch, scales, scale_pitch, col_blocks);
-    else if (rows * cols * sizeof(T) > (128ull << 20))
-        hipLaunchKernelGGL((quantize_blocks_kernel<T, true>), dim3((unsigned)groups), dim3(256), 0, s->stream, static_cast<const T *>(x), pitch,
-                           rows, cols, static_cast<uint8_t *>(q), q_pitch, scales, scale_pitch, col_blocks);
-    else
-        hipLaunchKernelGGL((quantize_blocks_kernel<T, false>), dim3((unsigned)groups), dim3(256), 0, s->stream, static_cast<const T *>(x), pitch,
-                           rows, cols, static_cast<uint8_t *>(q), q_pitch, scales, scale_pitch, col_blocks);
+    const bool stream = rows * cols * sizeof(T) > (128ull << 20);
+    auto kernel = block_rows == 1 ? (stream ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>)
+                                  : (stream ? quantize_blocks_kernel<T, true> : quantize_blocks_kernel<T, false>);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), 0, s->stream, static_cast<const T *>(x), pitch, rows, cols,
+                       static_cast<uint8_t *>(q), q_pitch, scales, scale_pitch, col_blocks);
     return launch_status();
 }
 
