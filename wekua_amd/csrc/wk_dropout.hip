@@ -50,6 +50,8 @@ typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2))); // 1
 // begins at a multiple of four elements, so the PER words are whole blocks; otherwise a row's first word is
 // (row * cols) % 4 words into its block and one block more is drawn.  STREAM: the tensors are more than the last-level cache
 // holds (256 MB) and pass it by.
+// Bound by memory, with the words' multiplications close behind: 8192 x 8192 bf16 45 us each way (5.9 TB/s), 65 with plain loads
+// and stores; 16 x 1024 f32 2.5 us, a launch.
 template <typename T, int PER, bool PHASE0, bool STREAM>
 __global__ __launch_bounds__(256) void dropout_kernel(const T *x, T *y, DropArgs a, typename wide_of<T>::type scale, uint64_t chunks_per_row,
                                                       uint64_t chunks) {
