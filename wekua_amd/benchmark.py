@@ -6,6 +6,7 @@ times over 1-D sizes, on GPU 0.
     python -m wekua_amd.benchmark axpy [--dtype f32]
     python -m wekua_amd.benchmark configs        # every GEMM / AXPY benchmark configuration, one line each
     python -m wekua_amd.benchmark tensor         # transpose / copy / random.uniform / toComplex streaming rates
+    python -m wekua_amd.benchmark tokens [--rows 1 8 2048] [--hidden 4096] [--vocab 32000] [--top 20]   # the operators at the token end
     python -m wekua_amd.benchmark probe          # cost of an empty and of a store-only launch on the GEMM grids
     python -m wekua_amd.benchmark mlp [--dtype f32] [--sizes 1024 4096 4096 1024] [--batch 2048] [--optimizer adam]
 
@@ -417,6 +418,48 @@ def cmd_tensor(ses, args):
         t.release(ses.pipeline)
 
 
+def cmd_tokens(ses, args):
+    """The operators at the token end of a network, as a serving and a training pass chain them: quantise, 8-bit product into
+    logits, log probabilities with alternatives and their gradient, dropout on the way back."""
+    wk, pipeline, ctx, lib = ses.wk, ses.pipeline, ses.ctx, ses.lib
+    K, V, top = args.hidden, args.vocab, args.top
+
+    def show(what, ms, nbytes, flops=0):
+        print(f"{what:58s} {ms * 1e3:9.1f} us  {nbytes / ms / 1e9:6.2f} TB/s" + (f"  {flops / ms / 1e9:7.1f} TFLOP/s" if flops else ""))
+    w = ses.tensor_on_device("f32", (V, K), 1)
+    qw = wk.blas.BlockScaled.init(ctx, pipeline, V, K, 128)
+    show(f"quantize weights {V} x {K} f32", ses.time_ms(lambda: qw.quantize(pipeline, w), 20), 5 * V * K)
+    w.release(pipeline)
+    for rows in args.rows:
+        x = ses.tensor_on_device("f32", (rows, K), 2)
+        qx = wk.blas.BlockScaled.init(ctx, pipeline, rows, K, 1)
+        show(f"quantize rows {rows} x {K} f32", ses.time_ms(lambda: qx.quantize(pipeline, x), 50), 5 * rows * K)
+        for dtype, size in (("bf16", 2), ("f32", 4)):
+            logits = wk.Tensor.alloc(dtype, ctx, pipeline, (rows, V))
+            show(f"gemmF8 {rows} x {V} x {K} {dtype}", ses.time_ms(lambda: wk.blas.gemmF8(pipeline, qx, qw, None, -1, logits), 20),
+                 (rows + V) * K + size * rows * V, 2 * rows * V * K)
+            for n in sorted({0, top}):
+                state = wk.nn.TokenLogProbs.init(dtype, ctx, pipeline, rows, V, n)
+                show(f"TokenLogProbs.forward {rows} x {V} {dtype}, {n} alternatives",
+                     ses.time_ms(lambda: state.forward(pipeline, logits), 20), size * rows * V)
+                if n:
+                    state.deinit(pipeline)
+                    continue
+                grad = wk.Tensor.alloc(dtype, ctx, pipeline, (rows, V))
+                targets = ses.tensor("i32", np.arange(rows, dtype=np.int32) % V)
+                show(f"TokenLogProbs.backward {rows} x {V} {dtype}",
+                     ses.time_ms(lambda: state.backward(pipeline, logits, targets, state.lse, None, grad), 20), 2 * size * rows * V)
+                for t in (grad, targets):
+                    t.release(pipeline)
+                state.deinit(pipeline)
+            show(f"dropout in place {rows} x {V} {dtype}", ses.time_ms(lambda: wk.random.dropout(pipeline, logits, logits, 0.1, 3), 20),
+                 2 * size * rows * V)
+            logits.release(pipeline)
+        x.release(pipeline)
+        qx.deinit(pipeline)
+    qw.deinit(pipeline)
+
+
 def mlp_flops(sizes, batch):
     """Multiply-adds of the GEMMs of one training step, as flops: forward and weight gradients over
     every layer, input sensitivities over every layer but the first."""
@@ -545,6 +588,11 @@ def main(argv=None):
     a = sub.add_parser("axpy")
     a.add_argument("--dtype", default="f32")
     sub.add_parser("tensor")
+    t = sub.add_parser("tokens")
+    t.add_argument("--rows", type=int, nargs="+", default=[1, 8, 2048])
+    t.add_argument("--hidden", type=int, default=4096)
+    t.add_argument("--vocab", type=int, default=32000)
+    t.add_argument("--top", type=int, default=20)
     r = sub.add_parser("regret")
     r.add_argument("--dtype", default="f32", choices=["f32", "f64"])
     r.add_argument("--ks", type=int, nargs="+", default=[384, 1024, 2500, 6000])
@@ -571,7 +619,7 @@ def main(argv=None):
     try:
         if getattr(args, "variant", "auto") != "auto":
             raw.check(ses.lib.wk_gemm_force_variant(args.variant.encode()), "wk_gemm_force_variant")
-        {"gemm": cmd_gemm, "axpy": cmd_axpy, "configs": cmd_configs, "tensor": cmd_tensor, "probe": cmd_probe, "narrow": cmd_narrow, "regret": cmd_regret}[args.cmd](ses, args)
+        {"gemm": cmd_gemm, "axpy": cmd_axpy, "configs": cmd_configs, "tensor": cmd_tensor, "tokens": cmd_tokens, "probe": cmd_probe, "narrow": cmd_narrow, "regret": cmd_regret}[args.cmd](ses, args)
     finally:
         ses.close()
     return 0
