@@ -48,10 +48,10 @@ typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2))); // 1
 
 // One thread takes PER consecutive elements of a row, 16 bytes (f64: 32), loaded before their words are drawn.  PHASE0: every row
 // begins at a multiple of four elements, so the PER words are whole blocks; otherwise a row's first word is
-// (row * cols) % 4 words into its block and one block more is drawn.  STREAM: the tensors are more than the last-level cache
-// holds (256 MB) and pass it by.
-// Bound by memory, with the words' multiplications close behind: 8192 x 8192 bf16 45 us each way (5.9 TB/s), 65 with plain loads
-// and stores; 16 x 1024 f32 2.5 us, a launch.
+// (row * cols) % 4 words into its block and one block more is drawn.  STREAM: the tensors fill the last-level cache (256 MB)
+// or more and pass it by.
+// Bound by memory, with the words' multiplications close behind: 8192 x 8192 bf16 43 us each way (6.2 TB/s), 45 with
+// plain loads and stores, 65 where the words were drawn first; 16 x 1024 f32 2.5 us, a launch.
 template <typename T, int PER, bool PHASE0, bool STREAM>
 __global__ __launch_bounds__(256) void dropout_kernel(const T *x, T *y, DropArgs a, typename wide_of<T>::type scale, uint64_t chunks_per_row,
                                                       uint64_t chunks) {
@@ -138,7 +138,7 @@ template <typename T> int dropout_launch(wk_stream *s, const void *x, void *y, D
     const W scale = p < 1.0 ? (W)(1.0 / (1.0 - p)) : W(0);
     const uint64_t per_row = (a.cols + PER - 1) / PER, chunks = per_row * a.total_rows;
     if ((chunks + 255) / 256 > most_groups(256)) return WK_E_INVALID_VALUE;
-    const bool phase0 = a.total_rows == 1 || a.cols % 4 == 0, stream = 2 * a.total_rows * a.cols * sizeof(T) > (256ull << 20);
+    const bool phase0 = a.total_rows == 1 || a.cols % 4 == 0, stream = 2 * a.total_rows * a.cols * sizeof(T) >= (256ull << 20);
     if (phase0) (stream ? dropout_enqueue<T, PER, true, true> : dropout_enqueue<T, PER, true, false>)(s->stream, chunks, per_row, x, y, a, scale);
     else (stream ? dropout_enqueue<T, PER, false, true> : dropout_enqueue<T, PER, false, false>)(s->stream, chunks, per_row, x, y, a, scale);
     return launch_status();
