@@ -226,8 +226,9 @@ template <bool ALIGNED, typename O> __global__ __launch_bounds__(256, 2) void ge
 // is in registers the wavefronts meet: the block is read, the next one has landed (it was asked for STAGES - 1 blocks ago), its stage is
 // asked to be filled again, and the next block's first operands are read while the last row of products still runs.
 //
-// 16-bit results, 8192^3: 510 us, 2.15 PFLOP/s (a library product of tensors with one scale 398); matrix instructions run 55 % of
-// the time at a clock that the power limit holds near 1.6 GHz.  f32: 1090 us, 1.0 PFLOP/s (the library's f16 product 770).  There the vector
+// 16-bit results, 8192^3: 510 us, 2.15 PFLOP/s (a library product of tensors with one scale 398); matrix instructions run half
+// of the time at a clock that the power limit holds near 1.9 GHz.  A block takes 4000 cycles: 2048 of products, and as many of the LDS port
+// (192 KB of operands to eight wavefronts, 64 KB that arrive; without the arrivals 428 us, without the barrier 500).  f32: 1090 us, 1.0 PFLOP/s (the library's f16 product 770).  There the vector
 // instructions are the bound: of 2400 cycles to a block of a 128 x 128 tile 1024 are products, and with them 128 widenings of
 // two codes at 8 cycles, 64 multiply-adds and what moves data have to be issued; taking turns with the products brought 2580 to
 // that.  Tiles of 128 x 256 widen a quarter less, but their sums do not fit the 256 registers that vector instructions reach.
