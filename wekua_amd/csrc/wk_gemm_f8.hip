@@ -92,19 +92,25 @@ __device__ __forceinline__ i32x4 first_bytes(i32x4 v, uint32_t n) {
     return v;
 }
 
-// 16 bytes of a row from byte k on; bytes at and beyond K are zero
-template <bool ALIGNED> __device__ __forceinline__ i32x4 load_chunk(const uint8_t *row, uint32_t k, uint32_t K) {
+typedef int i32x4_any __attribute__((ext_vector_type(4), aligned(1))); // 16 bytes at any address
+
+// 16 bytes of a row from byte k on; bytes at and beyond K are zero, and nothing there is read
+__device__ __forceinline__ i32x4 load_chunk(const uint8_t *row, uint32_t k, uint32_t K) {
+    if (k + 16 <= K) return *reinterpret_cast<const i32x4_any *>(row + k);
     i32x4 v = {0, 0, 0, 0};
     if (k >= K) return v;
-    const uint32_t left = K - k;
-    if (ALIGNED) {
-        v = *reinterpret_cast<const i32x4 *>(row + k);
-        if (left < 16) v = first_bytes(v, left);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-            if ((uint32_t)e < left) v[e / 4] |= (int)row[k + e] << (8 * (e % 4));
+    if (K >= 16) { // the row's last 16 bytes, moved down
+        v = *reinterpret_cast<const i32x4_any *>(row + K - 16);
+        const uint32_t down = 16 - (K - k);
+        if (down & 8) v = i32x4{v[2], v[3], 0, 0};
+        if (down & 4) v = i32x4{v[1], v[2], v[3], 0};
+        const uint32_t b = down & 3;
+        return i32x4{(int)__builtin_amdgcn_alignbyte(v[1], v[0], b), (int)__builtin_amdgcn_alignbyte(v[2], v[1], b),
+                     (int)__builtin_amdgcn_alignbyte(v[3], v[2], b), (int)__builtin_amdgcn_alignbyte(0, v[3], b)};
     }
+#pragma unroll
+    for (int e = 0; e < 15; ++e)
+        if (k + e < K) v[e / 4] |= (int)row[k + e] << (8 * (e % 4));
     return v;
 }
 
@@ -144,10 +150,12 @@ template <typename O, bool ACT = true> __device__ __forceinline__ void store_row
     }
 }
 
-// 128 x 128 tile of C, four wavefronts with 64 x 64 each; k-blocks go through registers into LDS, the next one's loads in
+// Operands off 16-byte boundaries (direct loads into LDS want those) or 2^23 and more apart: 128 x 128 tile of C, four wavefronts with 64 x 64
+// each; their 16-byte loads from any address are what bounds it where that is no multiple of 4 (1000 x 4095 x 4001 f32, rows 4001 apart
+// 114 us, byte by byte 521; 4016 apart, by the kernel below, 50).  k-blocks go through registers into LDS, the next one's loads in
 // flight while this one's products run.  Rows in LDS are 128 bytes; 16-byte chunk c of row r lies at c ^ (r % 8), so that
 // the eight lanes which LDS serves together read all its banks.
-template <bool ALIGNED, typename O> __global__ __launch_bounds__(256, 2) void gemm_f8_tile_kernel(F8Args a) {
+template <typename O> __global__ __launch_bounds__(256, 2) void gemm_f8_tile_kernel(F8Args a) {
     constexpr int TM = 128, TN = 128;
     __shared__ i32x4 la[TM * 8], lb[TN * 8];
     const uint32_t tiles_m = (a.M + TM - 1) / TM;
@@ -174,10 +182,12 @@ template <bool ALIGNED, typename O> __global__ __launch_bounds__(256, 2) void ge
     f32x4 acc[4][4] = {};
     i32x4 va[4], vb[4];
     auto fetch = [&](uint32_t kb) {
+        const bool inside = kb < a.K / KB;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            va[i] = load_chunk<ALIGNED>(pa[i], kb * KB + cc * 16, a.K);
-            vb[i] = load_chunk<ALIGNED>(pb[i], kb * KB + cc * 16, a.K);
+            const uint32_t k = kb * KB + cc * 16;
+            va[i] = inside ? *reinterpret_cast<const i32x4_any *>(pa[i] + k) : load_chunk(pa[i], k, a.K);
+            vb[i] = inside ? *reinterpret_cast<const i32x4_any *>(pb[i] + k) : load_chunk(pb[i], k, a.K);
         }
     };
     fetch(0);
@@ -560,7 +570,7 @@ template <typename O, int WM, int WN, int MT, int NT, int STAGES> int gemm_f8_dm
 // work-group take a block of k in turn, DEEP of them in flight each, and their sums meet in LDS in wavefront order.
 // Work-groups start their walk along k at different places: rows a power of two apart lie in the same memory channel, and all
 // work-groups would go through the channels in step.
-template <bool ALIGNED, typename O, int MT, int NT, int DEEP, uint32_t WAVES = 8> __global__ __launch_bounds__(WAVES * 64) void gemm_f8_rows_kernel(F8Args a) {
+template <typename O, int MT, int NT, int DEEP, uint32_t WAVES = 8> __global__ __launch_bounds__(WAVES * 64) void gemm_f8_rows_kernel(F8Args a) {
     __shared__ f32x4 part[WAVES][MT * NT][64];
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, r16 = lane % 16, g = lane / 16;
     const uint32_t n0 = blockIdx.x * (16 * NT), m0 = blockIdx.y * (16 * MT);
@@ -588,10 +598,10 @@ template <bool ALIGNED, typename O, int MT, int NT, int DEEP, uint32_t WAVES = 8
             const uint32_t k = kb * KB + h * 64 + g * 16;
 #pragma unroll
             for (int j = 0; j < NT; ++j)
-                cb[d][j][h] = inside && ALIGNED ? *reinterpret_cast<const i32x4 *>(pb[j] + k) : load_chunk<ALIGNED>(pb[j], k, a.K);
+                cb[d][j][h] = inside ? *reinterpret_cast<const i32x4_any *>(pb[j] + k) : load_chunk(pb[j], k, a.K);
 #pragma unroll
             for (int i = 0; i < MT; ++i)
-                ca[d][i][h] = inside && ALIGNED ? *reinterpret_cast<const i32x4 *>(pa[i] + k) : load_chunk<ALIGNED>(pa[i], k, a.K);
+                ca[d][i][h] = inside ? *reinterpret_cast<const i32x4_any *>(pa[i] + k) : load_chunk(pa[i], k, a.K);
         }
 #pragma unroll
         for (int i = 0; i < MT; ++i) sa[d][i] = psa[i][kb];
@@ -647,21 +657,21 @@ template <bool ALIGNED, typename O, int MT, int NT, int DEEP, uint32_t WAVES = 8
     }
 }
 
-template <bool ALIGNED, typename O, int MT, int NT, int DEEP, uint32_t WAVES = 8> int gemm_f8_rows_launch(hipStream_t st, const F8Args &a) {
+template <typename O, int MT, int NT, int DEEP, uint32_t WAVES = 8> int gemm_f8_rows_launch(hipStream_t st, const F8Args &a) {
     const uint32_t across = (a.N + 16 * NT - 1) / (16 * NT);
     if (across > most_groups(WAVES * 64)) return WK_E_INVALID_VALUE;
-    hipLaunchKernelGGL((gemm_f8_rows_kernel<ALIGNED, O, MT, NT, DEEP, WAVES>), dim3(across, (a.M + 16 * MT - 1) / (16 * MT)), dim3(WAVES * 64), 0, st, a);
+    hipLaunchKernelGGL((gemm_f8_rows_kernel<O, MT, NT, DEEP, WAVES>), dim3(across, (a.M + 16 * MT - 1) / (16 * MT)), dim3(WAVES * 64), 0, st, a);
     return launch_status();
 }
 
 // Up to 64 rows.  Measured (f32 results, us; N = K = 8192 unless said): 8 rows 16 columns at a time 19.5, 32 columns and sixteen
 // wavefronts 17.7, but 9.8 against 13.0 at N = 2048, where those leave three quarters of the units without work; 32 rows 32 at
 // a time 26.6 (16: 41); 64 rows 64 at a time 33.0 against 41.8 for 32, but 18.6 against 12.4 at N = K = 4096.
-template <bool ALIGNED, typename O> int gemm_f8_rows(hipStream_t st, const F8Args &a) {
+template <typename O> int gemm_f8_rows(hipStream_t st, const F8Args &a) {
     const bool wide = a.N >= 32 * 256; // a work-group of 32 columns for each unit
-    if (a.M <= 16) return wide ? gemm_f8_rows_launch<ALIGNED, O, 1, 2, ALIGNED ? 4 : 2, 16>(st, a) : gemm_f8_rows_launch<ALIGNED, O, 1, 1, 4>(st, a);
-    if (a.M <= 32 || !wide) return gemm_f8_rows_launch<ALIGNED, O, 2, 2, 2>(st, a);
-    return gemm_f8_rows_launch<ALIGNED, O, 4, 2, 2>(st, a);
+    if (a.M <= 16) return wide ? gemm_f8_rows_launch<O, 1, 2, 4, 16>(st, a) : gemm_f8_rows_launch<O, 1, 1, 4>(st, a);
+    if (a.M <= 32 || !wide) return gemm_f8_rows_launch<O, 2, 2, 2>(st, a);
+    return gemm_f8_rows_launch<O, 4, 2, 2>(st, a);
 }
 
 // Which tile: its launch's time by rounds of what is resident, from measured rounds of 64 blocks of k (us; 256 units) with one
@@ -692,7 +702,7 @@ template <typename O> int gemm_f8_launch(wk_stream *s, const F8Args &a, bool ali
     const bool direct = aligned && a.lda < (1u << 23) && a.ldb < (1u << 23) && a.sap < (1u << 21) && a.sbp < (1u << 21);
     // f32 results: 64 rows 33 us either way (N = K = 8192); 16-bit ones have tiles of 8-bit instructions from 17 rows on (64: 20 us, 32 rows in the
     // lanes 26)
-    if (a.M <= (direct && !std::is_same_v<O, float> ? 16 : 64)) return aligned ? gemm_f8_rows<true, O>(st, a) : gemm_f8_rows<false, O>(st, a);
+    if (a.M <= (direct && !std::is_same_v<O, float> ? 16 : 64)) return gemm_f8_rows<O>(st, a);
     if (direct) {
         if constexpr (std::is_same_v<O, float>) {
             constexpr TileTime t[] = {{128, 128, 2, 79, 148}, {64, 128, 2, 50, 85}, {64, 64, 2, 34, 51}};
@@ -715,10 +725,7 @@ template <typename O> int gemm_f8_launch(wk_stream *s, const F8Args &a, bool ali
     }
     const uint64_t tiles = (uint64_t)((a.M + 127) / 128) * ((a.N + 127) / 128);
     if (tiles > most_groups(256)) return WK_E_INVALID_VALUE;
-    if (aligned)
-        hipLaunchKernelGGL((gemm_f8_tile_kernel<true, O>), dim3((unsigned)tiles), dim3(256), 0, st, a);
-    else
-        hipLaunchKernelGGL((gemm_f8_tile_kernel<false, O>), dim3((unsigned)tiles), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(gemm_f8_tile_kernel<O>, dim3((unsigned)tiles), dim3(256), 0, st, a);
     return launch_status();
 }
 
