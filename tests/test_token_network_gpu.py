@@ -145,6 +145,28 @@ def test_block_scaled_product(env, dtype, M, N, K, kind):
     release(env, tx, tw, tb, c)
 
 
+@pytest.mark.parametrize("rows,n,k", [(5, 130, 300), (150, 260, 129)])
+def test_product_with_the_weights_turned_around(env, rows, n, k):
+    """The gradient of a layer's input: the same codes and scales, transposed, under the quantised gradient of its output."""
+    context, pipeline = env
+    rng = np.random.RandomState(n)
+    w, g = rng.randn(n, k).astype(np.float32), rng.randn(rows, n).astype(np.float32)
+    tw, tg, out = upload(env, "f32", w), upload(env, "f32", g), Tensor.alloc("f32", context, pipeline, (rows, k))
+    init = wk.blas.BlockScaled.init
+    b, turned, a = init(context, pipeline, n, k, 128), init(context, pipeline, k, n, 128), init(context, pipeline, rows, n, 1)
+    b.quantize(pipeline, tw)
+    a.quantize(pipeline, tg)
+    wk.transpose(pipeline, turned.codes, b.codes, 0, 1)
+    wk.transpose(pipeline, turned.scales, b.scales, 0, 1)
+    wk.blas.gemmF8(pipeline, a, turned, None, -1, out)
+    codes, scales = ot.f8_quantize(w.astype(np.float64), 128)
+    want, mag, _ = ot.gemm_f8(*ot.f8_quantize(g.astype(np.float64), 1), np.ascontiguousarray(codes.T), np.ascontiguousarray(scales.T))
+    assert (np.abs(download(env, out) - want) <= (n + 8) * 2.0 ** -24 * mag).all()
+    for m in (a, b, turned):
+        m.deinit(pipeline)
+    release(env, tw, tg, out)
+
+
 def test_block_scaled_refusals(env):
     context, pipeline = env
     for rows, cols, block in ((0, 4, 1), (4, 0, 1), (4, 4, 2), (4, 4, 0)):

@@ -254,7 +254,7 @@ def test_gradient_of_the_kernels_own_statistics_against_differences(dev):
 def test_refusals(dev):
     lib, b = dev.lib, dev.malloc(1 << 16)
     p = b.ptr.value
-    base = dict(dtype=8, rows=2, vocab=8, x=p, pitch=8, t=p + 1024, tt=4, lp=p + 2048, lse=p + 3072, ent=p + 4096, top=2, ids=p + 5120, tl=p + 6144,
+    base = dict(dtype=8, rows=2, vocab=8, x=p, pitch=8, t=p + 1024, tt=4, lp=p + 2048, lse=p + 3200, ent=p + 4096, top=2, ids=p + 5120, tl=p + 6144,
                 ws=None, n=0)
 
     def call(stream=dev.stream, **change):
@@ -266,7 +266,7 @@ def test_refusals(dev):
     assert call(stream=None) == 1
     for bad in ({"dtype": 4}, {"dtype": 34}, {"dtype": 18}, {"dtype": 20}, {"tt": 5}, {"tt": 8}):
         assert call(**bad) == 9, bad
-    g = dict(dtype=8, rows=2, vocab=8, x=p, pitch=8, t=p + 1024, tt=4, lse=p + 2048, ent=p + 3072, w=p + 4096, h=p + 5120, g=p + 6144, gp=8)
+    g = dict(dtype=8, rows=2, vocab=8, x=p, pitch=8, t=p + 1024, tt=4, lse=p + 2048, ent=p + 3200, w=p + 4096, h=p + 5120, g=p + 6144, gp=8)
 
     def grad(stream=dev.stream, **change):
         return lib.wk_token_logprobs_grad(stream, *{**g, **change}.values())
