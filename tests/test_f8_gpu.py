@@ -116,6 +116,13 @@ def test_gemm_large(dev, out, M, N, K, kind):
     check_gemm(dev, M, N, K, out, kind == 0, kind, pads=(-K % 16, -K % 16, 4 if M % 2 else 0), cut=False)
 
 
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("M,N,K", [(1, 16384, 140), (8, 16421, 256), (17, 16383, 300), (33, 20000, 130), (32, 32768, 64), (64, 33000, 133), (40, 33000, 300), (5, 70001, 129)])
+def test_gemm_few_rows_many_columns(dev, out, M, N, K):
+    """Both sides of where tiles take over from streaming, and between tiles of 64 and 128 columns."""
+    check_gemm(dev, M, N, K, out, True, 1, pads=(-K % 16, -K % 16, 0), cut=False)
+
+
 @pytest.mark.parametrize("out", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("bias,kind", [(False, -1), (True, -1), (True, 0), (False, 1)])
 @pytest.mark.parametrize("M,N", [(3, 70), (200, 300)])

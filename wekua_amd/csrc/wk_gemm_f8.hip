@@ -700,11 +700,16 @@ template <typename O> int gemm_f8_launch(wk_stream *s, const F8Args &a, bool ali
     const hipStream_t st = s->stream;
     // the loads into LDS have lane offsets of 32 bits within a tile
     const bool direct = aligned && a.lda < (1u << 23) && a.ldb < (1u << 23) && a.sap < (1u << 21) && a.sbp < (1u << 21);
-    // f32 results: 64 rows 33 us either way (N = K = 8192); 16-bit ones have tiles of 8-bit instructions from 17 rows on (64: 20 us, 32 rows in the
-    // lanes 26)
-    if (a.M <= (direct && !std::is_same_v<O, float> ? 16 : 64)) return gemm_f8_rows<O>(st, a);
+    // Few rows: the kernel above while tiles would leave units idle (8 x 8192 x 8192 f32 18 us, in tiles 30; 8 x 2048 x 8192 10 against
+    // 29), tiles of 64 rows from one for every unit on (8 x 28672 x 8192 66 against 52, 17 x 65536 x 512 16 against 12; 8 x 32000 x 4096 32
+    // either way).  16-bit results have the faster tiles: from 17 rows on wherever (17 x 8192 x 8192 28 against 22, 17 x 2048 x 8192 17 either way).
+    constexpr bool WIDE = std::is_same_v<O, float>;
+    if (a.M <= 64 && !(direct && (a.N >= 64 * 256 || (!WIDE && a.M > 16)))) return gemm_f8_rows<O>(st, a);
+    // one row of tiles waits for memory, and small ones ask for more at a time (8 x 28672 x 8192 bf16 46 us, with 64 x 128 53; f32 52 and 55, but
+    // 64 rows, bound by their widening, 66 and 57)
+    if (direct && a.M <= (WIDE ? 32 : 64) && a.N <= 64 * 512) return gemm_f8_dma_launch<O, 2, 2, 2, 2, 4>(st, a);
     if (direct) {
-        if constexpr (std::is_same_v<O, float>) {
+        if constexpr (WIDE) {
             constexpr TileTime t[] = {{128, 128, 2, 79, 148}, {64, 128, 2, 50, 85}, {64, 64, 2, 34, 51}};
             switch (best_tile(t, 3, a)) {
             case 0: return gemm_f8_dma_launch<O, 2, 2, 4, 4, 2>(st, a);
