@@ -81,7 +81,7 @@ void gemm_f64_dma_kernel(DArgsD g) {
     constexpr int CPR = BK / 2;   // 16-byte chunks per row of a k-contiguous slab
     constexpr int A_DOUBLES = BM * BK, B_DOUBLES = BN * BK, STAGE = A_DOUBLES + B_DOUBLES;
     constexpr int A_LOADS = BM * BK / 512, B_LOADS = BN * BK / 512; // 1 KB = 128 doubles per wavefront and load
-    static_assert(BK == 16 && BM % 32 == 0 && BN % 32 == 0 && A_LOADS >= 1 && B_LOADS >= 1, "tile shape");
+    static_assert(BK == 16 && BM % 32 == 0 && BN % 32 == 0 && A_LOADS >= 1 && B_LOADS >= 1 && A_LOADS % 2 == 0 && B_LOADS % 2 == 0, "tile shape");
 
     extern __shared__ __align__(16) float lds_f[];
     double *lds = reinterpret_cast<double *>(lds_f); // [NS][STAGE]: A then B
@@ -174,9 +174,9 @@ void gemm_f64_dma_kernel(DArgsD g) {
         const uint32_t sbase = lds0 + stage_bytes + (uint32_t)wave * 1024u;
         if constexpr (VB == 16) {
 #pragma unroll
-            for (int i = 0; i < A_LOADS; ++i) dma16(a_base, a_off[i], sbase + (uint32_t)i * 4096u);
+            for (int i = 0; i < A_LOADS; i += 2) dma16_pair<4096>(a_base, a_off[i], a_off[i + 1], sbase + (uint32_t)i * 4096u);
 #pragma unroll
-            for (int i = 0; i < B_LOADS; ++i) dma16(b_base, b_off[i], sbase + A_DOUBLES * 8u + (uint32_t)i * 4096u);
+            for (int i = 0; i < B_LOADS; i += 2) dma16_pair<4096>(b_base, b_off[i], b_off[i + 1], sbase + A_DOUBLES * 8u + (uint32_t)i * 4096u);
         } else {
 #pragma unroll
             for (int i = 0; i < A_LOADS * SUB; ++i) dma4(a_base, a_off[i], sbase + (uint32_t)(i / SUB) * 4096u + (uint32_t)(i % SUB) * 256u);
