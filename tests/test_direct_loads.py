@@ -46,3 +46,11 @@ def test_the_scan_sees_short_bases():
     assert check_main_loops.short_bases(written + "\ts_nop 4\n" + load) == (1, [])
     assert check_main_loops.short_bases(written + "\ts_mov_b64 s[6:7], s[4:5]\n\tglobal_load_lds_dword v0, s[6:7]\n") == (1, [])
     assert check_main_loops.short_bases("\tv_mov_b32_e32 v4, v5\n\tglobal_load_lds_dwordx4 v[4:5], off\n") == (1, [])
+
+
+def test_every_source_with_direct_loads_is_looked_at():
+    """A file that issues them belongs to the script's list."""
+    listed = {src for src, _ in check_main_loops.FILES}
+    for name in os.listdir(build.CSRC):
+        if name.endswith(".hip") and any(call in open(os.path.join(build.CSRC, name)).read() for call in ("dma16(", "dma4(", "global_load_lds")):
+            assert name in listed, name

@@ -21,12 +21,13 @@ from . import build
 
 FILES = [("wk_gemm_dma.hip", "gemm_f32_dma_kernel"), ("wk_gemm_dma_f64.hip", "gemm_f64_dma_kernel"),
          ("wk_gemm_ipack.hip", "gemm_i32_packed_dma_kernel"), ("wk_gemm_ipack.hip", "gemm_i8_packed_dma_kernel"),
-         ("wk_gemm_ipack.hip", "gemm_i16_packed_dma_kernel"), ("wk_gemm_i64pack.hip", "gemm_i64_packed_kernel")]
+         ("wk_gemm_ipack.hip", "gemm_i16_packed_dma_kernel"), ("wk_gemm_i64pack.hip", "gemm_i64_packed_kernel"),
+         ("wk_gemm_f8.hip", "gemm_f8_dma_kernel")]
 BASE_WAIT_STATES = 5    # between a vector instruction's write of a scalar register and a memory instruction's read of it
 
 
 def assembly(src: str, out: str) -> None:
-    flags = [f for f in build.HIP_FLAGS if f != "-fPIC"]
+    flags = [f for f in build.HIP_FLAGS if f != "-fPIC"] + build.SOURCE_FLAGS.get(src, [])
     subprocess.run([build.HIPCC] + flags + ["--cuda-device-only", "-S", os.path.join(build.CSRC, src), "-o", out],
                    check=True, stdout=subprocess.DEVNULL, stderr=subprocess.DEVNULL)
 
