@@ -6,6 +6,8 @@ added to the running sum (one rounding of 2^-24 per block): (128 + kblocks + 2) 
 16-bit results seven of eight consecutive products may each lose 2^-13 of the largest of them.  Then the bias
 (2^-24 of the result and of the sum before it), an activation (slope at most one; tanh and exp within 2^-20), and half a
 step of the result's type."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -128,6 +130,25 @@ def test_gemm_few_rows_many_columns(dev, out, M, N, K):
 @pytest.mark.parametrize("M,N", [(3, 70), (200, 300)])
 def test_gemm_epilogue(dev, out, bias, kind, M, N):
     check_gemm(dev, M, N, 272, out, bias, kind, pads=(0, 0, 1))
+
+
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("M,N,K", [(3, 70, 272), (200, 300, 272), (200, 300, 271), (2048, 520, 128)])
+def test_gemm_activation_is_the_element_wise_one(dev, kind, M, N, K):
+    """f32 results under an activation are, bit for bit, the plain results that the element-wise activation then runs over: few rows, tiles,
+    and operands off 16 bytes; sums from 0 to far where both saturate."""
+    rng = np.random.RandomState(M + kind)
+    a, b = (ot.e4m3_encode(np.clip(rng.randn(r, K) * 60, -448, 448)) for r in (M, N))
+    kb = -(-K // 128)
+    sa = (np.exp(3 * rng.randn(M, kb)) / 6000).astype(np.float32)
+    bufs = [dev.upload(v) for v in (a, b, sa, np.full((-(-N // 128), kb), 1 / 60, np.float32), rng.randn(N).astype(np.float32))]
+    plain, fused = dev.malloc(4 * M * N), dev.malloc(4 * M * N)
+    for c, k in ((plain, -1), (fused, kind)):
+        dev.gemm_f8(M, N, K, bufs[0], K, bufs[2], kb, bufs[1], K, bufs[3], kb, "f32", c, N, bufs[4], k)
+    assert dev.lib.wk_activation(dev.stream, 8, kind, (ctypes.c_uint64 * 3)(1, M, N), plain.ptr, N, M * N) == 0
+    assert np.array_equal(fused.download(np.uint32, (M, N)), plain.download(np.uint32, (M, N)))
+    for x in bufs + [plain, fused]:
+        x.free()
 
 
 @pytest.mark.parametrize("shift", [1, 4, 8])
