@@ -129,3 +129,27 @@ def test_refusals(dev):
         assert call(dtype=dtype) == 9, dtype
     dev.sync()
     b.free()
+
+
+def test_slices_of_one_row(dev):
+    """The row pitch of a single row is not walked and may be anything; slices that would lie over each other are refused all the
+    same, and so are pitches whose product passes 64 bits."""
+    cols = 40
+    x = np.arange(1, 3 * cols + 1, dtype=np.float32)
+    bx, by = dev.upload(x), dev.upload(np.full(3 * cols, -7, np.float32))
+    lib, s3 = dev.lib, ctypes.c_uint64 * 3
+
+    def call(shape, xrp, xsp, yrp, ysp):
+        return lib.wk_dropout(dev.stream, 8, s3(*shape), bx.ptr, xrp, xsp, by.ptr, yrp, ysp, 0.25, 6, 0, None)
+    for xrp, xsp, yrp, ysp in ((0, cols, 0, cols - 1), (0, cols - 1, 0, cols), (0, 0, cols, cols), (cols, cols, 0, 0), (1, 1, 1, 1)):
+        assert call((3, 1, cols), xrp, xsp, yrp, ysp) == 1, (xrp, xsp, yrp, ysp)
+    assert call((2, 2, 8), 2 ** 63, 0, 8, 16) == 1 and call((2, 2, 8), 8, 16, 2 ** 63, 0) == 1
+    assert (by.download(np.float32, (3 * cols,)) == -7).all()
+    want = ot.dropout(x.astype(np.float64), 0.25, 6, 0)
+    for pitch in (0, 1, cols, 2 ** 63):
+        by.write(np.full(3 * cols, -7, np.float32))
+        assert call((3, 1, cols), pitch, cols, pitch, cols) == 0
+        got = by.download(np.float32, (3 * cols,)).astype(np.float64)
+        assert np.array_equal(got == 0, want == 0) and close("f32", got, want)
+    for b in (bx, by):
+        b.free()

@@ -154,11 +154,16 @@ extern "C" int wk_dropout(wk_stream *s, int dtype, const uint64_t shape3[3], con
     const uint64_t depth = shape3[0], rows = shape3[1], cols = shape3[2];
     uint64_t n;
     if (__builtin_mul_overflow(depth, rows, &n) || __builtin_mul_overflow(n, cols, &n) || n >> 60) return WK_E_INVALID_VALUE;
-    if (rows > 1 && (xrp < cols || yrp < cols)) return WK_E_INVALID_VALUE;
-    if (depth > 1 && (xsp < rows * xrp || ysp < rows * yrp)) return WK_E_INVALID_VALUE;
     if (!(p >= 0.0 && p <= 1.0)) return WK_E_INVALID_VALUE;
-    if (rows == 1) xrp = yrp = cols; // pitches of dimensions of one are never walked
-    if (depth == 1) xsp = rows * xrp, ysp = rows * yrp;
+    // rows lie apart, and slices; pitches of dimensions of one are never walked, whatever they are
+    auto lay_apart = [&](uint64_t &rp, uint64_t &sp) {
+        if (rows == 1) rp = cols;
+        uint64_t slice;
+        if (rp < cols || __builtin_mul_overflow(rows, rp, &slice)) return false;
+        if (depth == 1) sp = slice;
+        return sp >= slice;
+    };
+    if (!lay_apart(xrp, xsp) || !lay_apart(yrp, ysp)) return WK_E_INVALID_VALUE;
     if (x == y && (xrp != yrp || xsp != ysp)) return WK_E_INVALID_VALUE;
     const double t = std::floor(p * 4294967296.0);
     DropArgs a{rows, cols, depth * rows, xrp, xsp, yrp, ysp, seed, offset, dev_step, (uint32_t)(t < 4294967295.0 ? t : 4294967295.0), t >= 4294967296.0};
