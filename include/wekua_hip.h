@@ -362,8 +362,8 @@ int  wk_token_logprobs(wk_stream *s, int dtype, uint64_t rows, uint64_t vocab, c
  *   logits_grad_j = logprob_grad * ((j == target) - p_j) - entropy_grad * p_j * (x_j - lse + entropy)
  * with one value of logprob_grad and entropy_grad to a row (f32, f64 for f64 logits); either may be NULL (targets too without
  * the first, entropy without the second), not both.  logits_grad is of the logits' type and may be logits itself
- * (same pitch).  A row without a target has no first term; masked logits get 0 (the target itself: logprob_grad); a row with
- * lse -inf gets zeros, one with a target that is not below vocab, or whose lse is NaN, gets NaN. */
+ * (same pitch).  A row without a target has no first term; masked logits get 0 (the target itself: logprob_grad).  A row gets NaN
+ * whose lse is NaN or, with logprob_grad, whose target is not below vocab; of the others one with lse -inf gets zeros. */
 int  wk_token_logprobs_grad(wk_stream *s, int dtype, uint64_t rows, uint64_t vocab, const void *logits, uint64_t pitch,
                             const void *targets, int target_dtype, const void *lse, const void *entropy, const void *logprob_grad,
                             const void *entropy_grad, void *logits_grad, uint64_t grad_pitch);

@@ -226,6 +226,28 @@ def test_gradient(dev, dtype, rows, vocab, pad, terms):
         b.free()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f64", "f16", "bf16"])
+@pytest.mark.parametrize("vocab", [5, 300, 9001])
+def test_gradient_of_empty_rows_and_no_tokens(dev, dtype, vocab):
+    """Rows that their mask leaves empty, whose target is a token, none, and not below vocab: zeros, zeros, NaN with a gradient of the
+    log probability, and always zeros without one; what forward answers for them beside it."""
+    acc = np.float64 if dtype == "f64" else np.float32
+    x = np.full((4, vocab), -np.inf)
+    targets = np.array([vocab - 1, -1, vocab, 2 ** 31 - 1])
+    bits = pack(dtype, x)
+    o = run_forward(dev, dtype, bits, targets, 0)
+    assert (o["lse"] == -np.inf).all() and (o["entropy"] == 0).all() and np.array_equal(o["logprob"], [-np.inf, 0, np.nan, np.nan], equal_nan=True)
+    up = [dev.upload(v) for v in (bits, targets.astype(np.int32), o["lse"], o["entropy"], np.array([np.nan, 3, 0, -1], acc), np.ones(4, acc))]
+    bg = dev.malloc(bits.nbytes)
+    for w, h in ((up[4], None), (up[4], up[5]), (None, up[5])):
+        dev.token_logprobs_grad(dtype, 4, vocab, up[0], vocab, up[1], "i32", up[2], up[3], w, h, bg, vocab)
+        got = values(dtype, bg.download(bits.dtype, bits.shape))
+        want = ot.token_logprobs_grad(x, targets, o["lse"], o["entropy"], None if w is None else np.array([np.nan, 3, 0, -1]), None if h is None else np.ones(4))
+        assert (got[:2] == 0).all() and (np.isnan(got[2:]).all() if w else (got[2:] == 0).all()) and np.array_equal(got, want, equal_nan=True)
+    for b in up + [bg]:
+        b.free()
+
+
 def test_gradient_of_the_kernels_own_statistics_against_differences(dev):
     """f64 logits: the gradient from the forward call's lse and entropy against central differences of the forward call."""
     rng = np.random.RandomState(21)

@@ -561,6 +561,7 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(const T *x, uint64_t
         ent = a.entropy[row];
     }
     const bool empty = lse == lowest(A(0));
+    const A none = t >= (int64_t)vocab ? A(__builtin_nanf("")) : A(0); // an empty row's gradient
 #pragma unroll
     for (int u = 0; u < GRAD_DEEP; ++u) {
         const uint32_t c = c0 + u * 256 * VE;
@@ -572,7 +573,7 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(const T *x, uint64_t
             A g = -w * p;
             if (ENTROPY) g -= h * mul0(p, d + ent);
             if (here && t == (int64_t)(c + e)) g += w;
-            raw[u][e] = (T)(empty ? A(0) : g);
+            raw[u][e] = (T)(empty ? none : g);
         }
         if (vocab - c >= (uint32_t)VE) {
             u32x4_any v;
