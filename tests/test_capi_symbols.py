@@ -295,3 +295,20 @@ def test_product_package_never_touches_the_oracle():
     for so in ("libwekua_hip.so", "libwekua_host.so"):
         out = subprocess.run(["ldd", os.path.join(pkg, so)], capture_output=True, text=True).stdout
         assert "oracle" not in out
+
+
+def test_types_of_every_operation():
+    """isTypeSupported answers for code that walks over types with any operation: the twenty, none of the formats that only a few
+    operations take; the same in Python and C++."""
+    from wekua_amd import CommandQueue, DTYPE_NAMES, EXTRA_DTYPES
+    queue = CommandQueue(None, 0)
+    assert len(DTYPE_NAMES) == 20 and all(queue.isTypeSupported(d) for d in DTYPE_NAMES)
+    assert not any(queue.isTypeSupported(d) for d in list(EXTRA_DTYPES) + ["f128", ""])
+    src = """#include "wekua.hpp"
+using namespace wekua::core;
+static_assert(CommandQueue::isTypeSupported<float>() && CommandQueue::isTypeSupported<uint64_t>() && CommandQueue::isTypeSupported<Complex<int8_t>>());
+static_assert(!CommandQueue::isTypeSupported<F16>() && !CommandQueue::isTypeSupported<BF16>() && !CommandQueue::isTypeSupported<F8E4M3>());
+"""
+    res = subprocess.run(["g++", "-std=c++20", "-fsyntax-only", "-I" + os.path.join(ROOT, "include"), "-I" + os.path.join(ROOT, "wekua_amd", "host"),
+                          "-x", "c++", "-"], input=src, text=True, capture_output=True)
+    assert res.returncode == 0, res.stderr

@@ -176,7 +176,8 @@ class CommandQueue:
         self.wekua_id = index
 
     def isTypeSupported(self, dtype: str) -> bool:
-        return dtype in DTYPE_NAMES or dtype in EXTRA_DTYPES
+        """Of the types that every operation takes; f16, bf16 and f8e4m3 are for the few that name them."""
+        return dtype in DTYPE_NAMES
 
 
 class Context:

@@ -139,7 +139,8 @@ struct CommandQueue {
     // OpenCL native widths here)
     uint32_t vector_widths[10] = {16, 16, 8, 8, 4, 4, 2, 2, 4, 2};
 
-    template <typename T> bool isTypeSupported() const { return true; }
+    // the types that every operation takes; the element formats beyond the twenty are for the few that name them
+    template <typename T> static constexpr bool isTypeSupported() { return !isExtraFormat<T>(); }
     template <typename T> uint32_t vectorWidth() const {
         if constexpr (isExtraFormat<T>()) return 16 / sizeof(T);
         else return vector_widths[getTypeId<T>()];
