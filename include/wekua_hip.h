@@ -328,7 +328,9 @@ int  wk_f8_quantize(wk_stream *s, int dtype, uint64_t rows, uint64_t cols, const
 /* C = act(A B^T + bias) of 8-bit operands (WK_F8E4M3), what Linear.forward computes:
  *   C[m][n] = act( sum over blocks b of k: a_scales[m][b] * b_scales[n / 128][b] * sum_{k in b} A[m][k] B[n][k]  + bias[n] )
  * A is M x K, B is N x K (a weight matrix as Linear keeps it), both row-major; blocks are 128 elements of k, the last
- * one shorter when K is no multiple.  Any f32 scales are taken, not only the quantiser's.  Sums are held in
+ * one shorter when K is no multiple.  Any f32 scales are taken, not only the quantiser's, whose products a_scale * b_scale f32 holds:
+ * that product comes first, so where it passes 2^128 it is infinite (and a block whose sum is 0 gives NaN), and below 2^-126 it
+ * loses bits.  (The quantiser's stay within while the operands' largest magnitudes multiply to at most 2^143.)  Sums are held in
  * 32 bits; C is f32, f16 or bf16 (out_dtype), rounded once.  For f32 every product enters its sum whole; for the 16-bit types
  * the 8-bit matrix instructions are used, which cut each product at 2^-13 of the largest of the eight consecutive ones that
  * it is summed with (1.5e-5 of a result on normally distributed operands, where a half step of bf16 is 4e-3 and of f16

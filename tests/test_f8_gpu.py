@@ -132,6 +132,34 @@ def test_gemm_epilogue(dev, out, bias, kind, M, N):
     check_gemm(dev, M, N, 272, out, bias, kind, pads=(0, 0, 1))
 
 
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("M,N,K,pad", [(5, 140, 700, 4), (130, 140, 700, 4), (130, 140, 700, 0), (300, 300, 640, 0)])
+def test_gemm_far_scales(dev, out, M, N, K, pad):
+    """Scales from 2^-126 to 2^127 whose products f32 holds, large ones against small ones, zero scales, and blocks of zeros under
+    products up to 2^127: a zero block adds nothing.  Tolerance as in check_gemm; every product of scales is a power of two here, so exact."""
+    rng = np.random.RandomState(M + K)
+    kb = -(-K // 128)
+    a, b = (ot.e4m3_encode(np.clip(rng.randn(r, K) * 60, -448, 448)) for r in (M, N))
+    e = np.array([126, -126, 90, -90, 0, 127])[:kb]                  # of A's scales, block by block; B's the other way
+    ea, eb = np.tile(e, (M, 1)), np.tile(-e, (-(-N // 128), 1))
+    ea[:, -1], eb[:, -1] = 127, 0                                    # a block of zeros under 2^127
+    ea[1::3] -= 2 * (ea[1::3] > -100)                                # rows apart
+    sa, sb = (2.0 ** ea).astype(np.float32), (2.0 ** eb).astype(np.float32)
+    sa[2, 0] = 0
+    a[:, 128 * (kb - 1):] = 0
+    a[M - 1, :128] = 0x80                                            # and one of -0 within another row
+    lda, ldb = K + pad, K + pad
+    bufs = [dev.upload(v) for v in (pitched(a, lda, 0x7F), pitched(b, ldb, 0x7F), sa, sb)]
+    bc = dev.malloc(4 * M * N)
+    dev.gemm_f8(M, N, K, bufs[0], lda, bufs[2], kb, bufs[1], ldb, bufs[3], kb, out, bc, N)
+    got = values(out, bc.download(np.float32 if out == "f32" else np.uint16, (M, N)))
+    want, mag, largest = ot.gemm_f8(a, sa, b, sb)
+    tol = (128 + kb) * 2.0 ** -23 * mag + (7 * 2.0 ** -13 * largest + 2.0 ** -8 * 1.01 * np.abs(want) if out != "f32" else 2.0 ** -24 * np.abs(want))
+    assert (np.abs(got - want) <= tol + 1e-37).all()
+    for x in bufs + [bc]:
+        x.free()
+
+
 @pytest.mark.parametrize("kind", [0, 1])
 @pytest.mark.parametrize("M,N,K", [(3, 70, 272), (200, 300, 272), (200, 300, 271), (2048, 520, 128)])
 def test_gemm_activation_is_the_element_wise_one(dev, kind, M, N, K):
