@@ -611,6 +611,28 @@ def test_offsets_beyond_32_bits(dev):
             b.free()
 
 
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+def test_aligned_rows_far_apart(dev, out):
+    """Operands and scales on 16-byte boundaries whose rows lie 2^25 and 2^26 bytes apart, results 2^24 elements: tiles with offsets beyond
+    32 bits, ragged on both sides, and a shorter last block."""
+    rng = np.random.RandomState(6)
+    m, n, k, kb = 140, 150, 400, 4
+    lda, ldb, ldc, sap = 2 ** 25, 2 ** 26 + 16, 2 ** 24, 2 ** 22
+    a, b = (ot.e4m3_encode(np.clip(rng.randn(r, k) * 60, -448, 448)) for r in (m, n))
+    sa, sb = np.exp(rng.randn(m, kb)).astype(np.float32) / 60, np.exp(rng.randn(2, kb)).astype(np.float32) / 60
+    size = 4 if out == "f32" else 2
+    ba, bb, bsa, bsb, bc = (dev.malloc(v) for v in (m * lda, n * ldb, 4 * m * sap, 4 * 2 * sap, size * m * ldc))
+    for buf, host, pitch in ((ba, a, lda), (bb, b, ldb), (bsa, sa, sap), (bsb, sb, sap)):
+        put(dev, buf, host, pitch)
+    dev.gemm_f8(m, n, k, ba, lda, bsa, sap, bb, ldb, bsb, sap, out, bc, ldc)
+    got = values(out, fetch(dev, bc, np.float32 if out == "f32" else np.uint16, (m, n), ldc))
+    want, mag, largest = ot.gemm_f8(a, sa, b, sb)
+    tol = (128 + kb + 2) * 2.0 ** -23 * mag + (7 * 2.0 ** -13 * largest + 2.0 ** -8 * 1.01 * np.abs(want) if out != "f32" else 2.0 ** -24 * np.abs(want))
+    assert (np.abs(got - want) <= tol).all()
+    for x in (ba, bb, bsa, bsb, bc):
+        x.free()
+
+
 def test_more_than_the_cache_holds(dev):
     """Sizes beyond which the kernels do not keep their tensors in the last-level cache, looked at in places."""
     rng = np.random.RandomState(5)

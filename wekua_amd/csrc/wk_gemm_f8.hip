@@ -136,8 +136,8 @@ template <typename O, bool ACT = true> __device__ __forceinline__ void store_row
     }
 }
 
-// Operands off 16-byte boundaries (direct loads into LDS want those) or 2^23 and more apart: 128 x 128 tile of C, four wavefronts with 64 x 64
-// each; their 16-byte loads from any address are what bounds it where that is no multiple of 4 (1000 x 4095 x 4001 f32, rows 4001 apart
+// Operands off 16-byte boundaries (direct loads into LDS want those): 128 x 128 tile of C, four wavefronts with 64 x 64 each;
+// their 16-byte loads from any address are what bounds it where that is no multiple of 4 (1000 x 4095 x 4001 f32, rows 4001 apart
 // 114 us, byte by byte 521; 4016 apart, by the kernel below, 50).  k-blocks go through registers into LDS, the next one's loads in
 // flight while this one's products run.  Rows in LDS are 128 bytes; 16-byte chunk c of row r lies at c ^ (r % 8), so that
 // the eight lanes which LDS serves together read all its banks.
@@ -682,10 +682,8 @@ uint32_t best_tile(const TileTime *t, uint32_t count, const F8Args &a) {
     return best;
 }
 
-template <typename O> int gemm_f8_launch(wk_stream *s, const F8Args &a, bool aligned) {
+template <typename O> int gemm_f8_launch(wk_stream *s, const F8Args &a, bool direct) {
     const hipStream_t st = s->stream;
-    // the loads into LDS have lane offsets of 32 bits within a tile
-    const bool direct = aligned && a.lda < (1u << 23) && a.ldb < (1u << 23) && a.sap < (1u << 21) && a.sbp < (1u << 21);
     // Few rows: the kernel above while tiles would leave units idle (8 x 8192 x 8192 f32 18 us, in tiles 30; 8 x 2048 x 8192 10 against
     // 29), tiles of 64 rows from one for every unit on (8 x 28672 x 8192 66 against 52, 17 x 65536 x 512 16 against 12; 8 x 32000 x 4096 32
     // either way).  16-bit results have the faster tiles: from 17 rows on wherever (17 x 8192 x 8192 28 against 22, 17 x 2048 x 8192 17 either way).
