@@ -290,7 +290,8 @@ __global__ __launch_bounds__(WM * WN * 64, (WM * WN == 4 && STAGES * (WM * MT + 
     // (a lane whose row lies behind the edge repeats its first one, the last row if that lies there too)
     const uint8_t *const from_a = a.A + (m0 + (EDGE && lrow > last_a ? last_a : lrow)) * a.lda + lchunk;
     const uint8_t *const from_b = a.B + (n0 + (EDGE && lrow > last_b ? last_b : lrow)) * a.ldb + lchunk;
-    // In the shorter last block the chunks behind K repeat the last one that has some of it (and are put to zero later).
+    // In the shorter last block the chunks behind K repeat the last one that has some of it (and are put to zero later); that one is
+    // read whole, up to 15 bytes behind K, which share its 16 bytes of memory.
     const uint32_t rest = a.K % KB, beyond = rest && lchunk > (rest - 1) / 16 * 16 ? lchunk - (rest - 1) / 16 * 16 : 0;
     // Scales: wavefront w brings 64 of A's, rows 64 w ..., in the order in which a lane will want them: place p of 16 MT rows holds row
     // (p % MT) * 16 + p / MT; the wavefronts that are left bring B's, one per 128 columns (all the same ones: a branch here would
