@@ -60,8 +60,8 @@ __global__ __launch_bounds__(256) void dropout_kernel(const T *x, T *y, DropArgs
     const uint64_t idx = blockIdx.x * 256ull + threadIdx.x;
     if (idx >= chunks) return;
     uint64_t row = 0, c = idx * PER;
-    if (a.total_rows > 1) {
-        row = (chunks >> 32) ? idx / chunks_per_row : (uint32_t)idx / (uint32_t)chunks_per_row;
+    if (a.total_rows > 1) { // (chunks are fewer than 2^32: the launch counts its threads)
+        row = (uint32_t)idx / (uint32_t)chunks_per_row;
         c = (idx - row * chunks_per_row) * PER;
     }
     uint64_t slice = 0, r = row;
