@@ -285,6 +285,33 @@ def test_dropout_layer(env, dtype):
     release(env, tx, tg, wrong)
 
 
+def test_a_refused_pass_leaves_the_dropout_layer_as_it_was(env):
+    """Between a forward pass and its backward pass: neither the mask of that pass nor the next pass's count moves."""
+    context, pipeline = env
+    x, g = np.random.RandomState(8).rand(2, 9, 21).astype(np.float32) + 1
+    layer = nn.Sequential.init("f32")
+    layer.append(nn.Dropout.init("f32", context, 21, 0.4, seed=5))
+    cache = nn.Cache.init(context, pipeline, 9, [layer])
+    lc, tx, tg, wrong = cache.getLayerCache(0), upload(env, "f32", x), Tensor.alloc("f32", context, pipeline, (9, 21)), Tensor.alloc("f32", context, pipeline, (9, 20))
+
+    def back(count):
+        memory.readFromBuffer(pipeline, layer.getSensitivity(lc), g)
+        layer.backward(pipeline, lc, tx, tg)
+        near(download(env, tg), ot.dropout(g.astype(np.float64), 0.4, 5, count), "f32")
+    near(download(env, layer.forward(pipeline, tx, lc)), ot.dropout(x.astype(np.float64), 0.4, 5, 0), "f32")
+    for training in (True, False):
+        layer.setTraining(training)
+        with pytest.raises(wk.WekuaError):
+            layer.forward(pipeline, wrong, lc)
+    back(0)
+    layer.setTraining(True)
+    near(download(env, layer.forward(pipeline, tx, lc)), ot.dropout(x.astype(np.float64), 0.4, 5, 1), "f32")
+    back(1)
+    cache.deinit(pipeline)
+    layer.deinit(pipeline)
+    release(env, tx, tg, wrong)
+
+
 def network(env, dtype, p, sizes=(24, 40, 301)):
     context, pipeline = env
     seq = nn.Sequential.init(dtype)

@@ -347,9 +347,12 @@ template <typename T> struct Dropout : Layer<T> {
     }
     TensorT *forward(Pipeline *pipeline, TensorT *input, void *cache) const override {
         DropoutCache *c = static_cast<DropoutCache *>(cache);
-        c->p = training ? p : 0.0;
-        c->count = training ? count.fetch_add(1) : 0;
-        random::dropout<T>(pipeline, input, c->output, c->p, seed, c->count);
+        helpers::eqlTensorsShape<T>(input, c->output); // a refused call takes no count
+        const double drops = training ? p : 0.0;
+        const uint64_t n = training ? count.fetch_add(1) : 0;
+        random::dropout<T>(pipeline, input, c->output, drops, seed, n);
+        c->p = drops; // (once the pass runs: until then the cache holds the last one's, which backward goes by)
+        c->count = n;
         return c->output;
     }
     TensorT *getSensitivity(const void *cache) const override { return static_cast<const DropoutCache *>(cache)->sensitivity; }
