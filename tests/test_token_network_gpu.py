@@ -572,6 +572,62 @@ def test_captured_run(dev):
     step.free()
 
 
+def test_captured_dropout_layer(env):
+    """A network's forward and backward pass in a graph: without a step the replays repeat their masks, with one that is moved by the
+    passes in a replay each has new ones, the backward pass the same; the program's own passes between them too."""
+    context, pipeline = env
+    rng = np.random.RandomState(11)
+    x, g = (rng.rand(9, 21) + 1 for _ in range(2))
+    layer, inner = nn.Sequential.init("f64"), nn.Sequential.init("f64")
+    inner.append(nn.Dropout.init("f64", context, 21, 0.4, seed=5))
+    layer.append(inner)
+    cache = nn.Cache.init(context, pipeline, 9, [layer])
+    lc, tx, tg, step = cache.getLayerCache(0), upload(env, "f64", x), Tensor.alloc("f64", context, pipeline, (9, 21)), upload(env, "u64", np.zeros(1, np.uint64))
+    memory.readFromBuffer(pipeline, layer.getSensitivity(lc), g)
+    bad = upload(env, "i64", np.zeros(1, np.int64))
+    with pytest.raises(wk.WekuaError):
+        layer.setStep(bad)
+    near(download(env, layer.forward(pipeline, tx, lc)), ot.dropout(x, 0.4, 5, 0), "f64")       # count 0, no step
+    layer.setStep(step)
+    hip = ctypes.CDLL("libamdhip64.so.7")
+    lib = wk._lib()
+    lib.wkz_context_stream.restype = ctypes.c_void_p
+    dev_lib = wk._capi.load()
+    queue = ctypes.c_void_p(lib.wkz_context_stream(context._h, 0))
+    dev_lib.wk_stream_native.restype = ctypes.c_void_p
+    stream = ctypes.c_void_p(dev_lib.wk_stream_native(queue))
+    pipeline.waitAndCleanup()
+    graph, run = ctypes.c_void_p(), ctypes.c_void_p()
+    assert hip.hipStreamBeginCapture(stream, 1) == 0
+    try:
+        out = layer.forward(pipeline, tx, lc)                                                     # count 1 + step
+        layer.backward(pipeline, lc, tx, tg)
+    finally:
+        rc = hip.hipStreamEndCapture(stream, ctypes.byref(graph))
+    assert rc == 0 and hip.hipGraphInstantiate(ctypes.byref(run), graph, None, None, 0) == 0
+    masks = []
+    for at in (0, 1, 2, 2):
+        memory.readFromBuffer(pipeline, step, np.array([at], np.uint64))
+        pipeline.waitAndCleanup()
+        wk.fill.zeroes(pipeline, tg)
+        assert hip.hipGraphLaunch(run, stream) == 0
+        y, dx = download(env, out), download(env, tg)
+        near(y, ot.dropout(x, 0.4, 5, 1 + at), "f64")
+        near(dx, ot.dropout(g, 0.4, 5, 1 + at), "f64")
+        masks.append(y != 0)
+    assert np.array_equal(masks[2], masks[3]) and not np.array_equal(masks[0], masks[1]) and not np.array_equal(masks[1], masks[2])
+    near(download(env, layer.forward(pipeline, tx, lc)), ot.dropout(x, 0.4, 5, 2 + 2), "f64")   # the host's next count, and the step
+    layer.setStep(None)
+    layer.backward(pipeline, lc, tx, tg)                                                          # goes by the pass it belongs to
+    near(download(env, tg), ot.dropout(g, 0.4, 5, 2 + 2), "f64")
+    near(download(env, layer.forward(pipeline, tx, lc)), ot.dropout(x, 0.4, 5, 3), "f64")
+    hip.hipGraphExecDestroy(run)
+    hip.hipGraphDestroy(graph)
+    cache.deinit(pipeline)
+    layer.deinit(pipeline)
+    release(env, tx, tg, step, bad)
+
+
 def put(dev, buf, host, pitch):
     """Row by row: `pitch` elements lie between them."""
     host = np.ascontiguousarray(host)

@@ -128,6 +128,7 @@ HOST_SIGNATURES = {
     "wkz_gemm_f8": (ci, [vp, vp, vp, vp, ci, vp]),
     "wkz_nn_dropout_init": (ci, [vp, ci, u64, ctypes.c_double, u64p, ctypes.POINTER(vp)]),
     "wkz_nn_layer_set_training": (ci, [vp, ci]),
+    "wkz_nn_layer_set_step": (ci, [vp, vp]),
     "wkz_nn_token_logprobs_init": (ci, [vp, vp, ci, u64, u64, ctypes.c_uint32, ctypes.POINTER(vp)]),
     "wkz_nn_token_logprobs_deinit": (ci, [vp, vp]),
     "wkz_nn_token_logprobs_tensor": (ci, [vp, ci, ctypes.POINTER(vp)]),

@@ -797,6 +797,17 @@ int wkz_nn_layer_set_training(void *layer, int on) {
         dispatch_real(h->dtype, [&]<typename T>() { static_cast<nn::Layer<T> *>(h->layer)->setTraining(on != 0); });
     });
 }
+// step: a one-element u64 tensor that stays the caller's, or NULL
+int wkz_nn_layer_set_step(void *layer, void *step) {
+    return guard([&] {
+        LayerHandle *h = static_cast<LayerHandle *>(layer);
+        TensorHandle *hs = static_cast<TensorHandle *>(step);
+        if (hs && hs->dtype != WK_U64) throw Error(WK_E_UNQUAL_TENSORS_ATTRIBUTE);
+        dispatch_real(h->dtype, [&]<typename T>() {
+            static_cast<nn::Layer<T> *>(h->layer)->setStep(hs ? static_cast<Tensor<uint64_t> *>(hs->tensor) : nullptr);
+        });
+    });
+}
 
 struct TokenLogProbsHandle {
     int dtype;

@@ -126,7 +126,9 @@ template <typename T> struct Layer {
     virtual void backward(Pipeline *pipeline, void *cache, TensorT *input, TensorT *input_gradient) const = 0;
     virtual std::vector<TensorT *> getGradients(const void *cache) const = 0;
     virtual std::vector<TensorT *> getBiasGradients(const void *cache) const = 0; // entries may be null
-    virtual void setTraining(bool) {} // no counterpart in the reference: what Dropout listens to
+    // no counterpart in the reference: what Dropout listens to
+    virtual void setTraining(bool) {}
+    virtual void setStep(Tensor<uint64_t> *) {}
 };
 
 // ---- Linear ------------------------------------------------------------------------------------
@@ -299,17 +301,22 @@ template <typename T> struct Linear : Layer<T> {
 // ---- Dropout -----------------------------------------------------------------------------------
 // No counterpart in the reference.  random::dropout between two layers, `width` columns: every forward pass takes the layer's
 // next count, which its cache keeps for the backward pass.  setTraining(false): the outputs are the inputs.
+// The count is the host's, so passes captured into a graph keep the one they had then, and replays would repeat their masks.
+// setStep: one element in device memory (the caller's; null: none) that the passes from then on add to their count when they run; a
+// program moves it between replays by the forward passes of the layer in one, and not between a forward pass and its backward pass.
 template <typename T> struct Dropout : Layer<T> {
     using TensorT = Tensor<T>;
     struct DropoutCache {
         TensorT *output = nullptr, *sensitivity = nullptr;
         uint64_t count = 0; // of the last forward pass
         double p = 0.0;     // what it dropped
+        Tensor<uint64_t> *step = nullptr; // what it added to the count
     };
     const Context *context = nullptr;
     uint64_t width = 0, seed = 0;
     double p = 0.0;
     bool training = true;
+    Tensor<uint64_t> *step = nullptr;
     mutable std::atomic<uint64_t> count{0};
 
     static Dropout *init(const Context *context, uint64_t width, double p, std::optional<uint64_t> seed = std::nullopt) {
@@ -322,6 +329,10 @@ template <typename T> struct Dropout : Layer<T> {
         return d;
     }
     void setTraining(bool on) override { training = on; }
+    void setStep(Tensor<uint64_t> *counter) override {
+        if (counter && counter->context != context) throw Error(WK_E_UNQUAL_TENSORS_CONTEXT);
+        step = counter;
+    }
     void deinit(Pipeline *) override { delete this; }
     TensorT *getCachedOutput(const void *cache) const override { return static_cast<const DropoutCache *>(cache)->output; }
     std::vector<TensorT *> getWeights() const override { return {}; }
@@ -350,15 +361,16 @@ template <typename T> struct Dropout : Layer<T> {
         helpers::eqlTensorsShape<T>(input, c->output); // a refused call takes no count
         const double drops = training ? p : 0.0;
         const uint64_t n = training ? count.fetch_add(1) : 0;
-        random::dropout<T>(pipeline, input, c->output, drops, seed, n);
+        random::dropout<T>(pipeline, input, c->output, drops, seed, n, step);
         c->p = drops; // (once the pass runs: until then the cache holds the last one's, which backward goes by)
         c->count = n;
+        c->step = step;
         return c->output;
     }
     TensorT *getSensitivity(const void *cache) const override { return static_cast<const DropoutCache *>(cache)->sensitivity; }
     void backward(Pipeline *pipeline, void *cache, TensorT *, TensorT *input_sensitivity) const override {
         DropoutCache *c = static_cast<DropoutCache *>(cache);
-        if (input_sensitivity) random::dropout<T>(pipeline, c->sensitivity, input_sensitivity, c->p, seed, c->count);
+        if (input_sensitivity) random::dropout<T>(pipeline, c->sensitivity, input_sensitivity, c->p, seed, c->count, c->step);
     }
     std::vector<TensorT *> getGradients(const void *) const override { return {}; }
     std::vector<TensorT *> getBiasGradients(const void *) const override { return {}; }
@@ -377,6 +389,9 @@ template <typename T> struct Sequential : Layer<T> {
     void append(Layer<T> *layer) { layers.push_back(layer); }
     void setTraining(bool on) override {
         for (Layer<T> *l : layers) l->setTraining(on);
+    }
+    void setStep(Tensor<uint64_t> *counter) override {
+        for (Layer<T> *l : layers) l->setStep(counter);
     }
     void deinit(Pipeline *pipeline) override {
         for (Layer<T> *l : layers) l->deinit(pipeline);

@@ -118,6 +118,14 @@ class Layer:
         """Of a Dropout, or of the Dropout layers in a Sequential: off, their outputs are their inputs."""
         _w._check(_w._lib().wkz_nn_layer_set_training(self._h, int(on)), "Layer.setTraining")
 
+    def setStep(self, step) -> None:
+        """Of a Dropout, or of the Dropout layers in a Sequential: a one-element u64 tensor (or None) that their passes from then on
+        add to their count when they run.  A program that replays captured passes, whose count stays what it was at the capture, moves it
+        between replays by the forward passes of a layer in one to get new masks, and not between a forward pass and its
+        backward pass.  The tensor lives as long as the layers use it."""
+        _w._check(_w._lib().wkz_nn_layer_set_step(self._h, step._h if step is not None else None), "Layer.setStep")
+        self._step = step
+
     def forward(self, pipeline, input_tensor, layer_cache):
         h = vp()
         _w._check(_w._lib().wkz_nn_layer_forward(self._h, pipeline._h, input_tensor._h, layer_cache, ctypes.byref(h)),
