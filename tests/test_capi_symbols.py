@@ -312,3 +312,26 @@ static_assert(!CommandQueue::isTypeSupported<F16>() && !CommandQueue::isTypeSupp
     res = subprocess.run(["g++", "-std=c++20", "-fsyntax-only", "-I" + os.path.join(ROOT, "include"), "-I" + os.path.join(ROOT, "wekua_amd", "host"),
                           "-x", "c++", "-"], input=src, text=True, capture_output=True)
     assert res.returncode == 0, res.stderr
+
+
+def test_missing_handles_are_refused():
+    """The host library's calls at the token end of a network without a handle that they need, which is what a layer has that was appended to
+    another and an object after its deinit: an error, no access."""
+    import wekua_amd
+    lib = wekua_amd._lib()
+    u64p, out = ctypes.POINTER(ctypes.c_uint64), ctypes.c_void_p()
+    some = ctypes.c_void_p(16)          # never looked at: another one is missing
+    calls = {"wkz_random_dropout": (some, some, some, 0.5, 1, 0, None), "wkz_block_scaled_init": (some, some, 4, 4, 1, ctypes.byref(out)),
+             "wkz_block_scaled_deinit": (some, some), "wkz_block_scaled_quantize": (some, some, some), "wkz_block_scaled_tensor": (some, 0, ctypes.byref(out)),
+             "wkz_gemm_f8": (some, some, some, None, -1, some), "wkz_nn_dropout_init": (some, 8, 4, 0.5, u64p(), ctypes.byref(out)),
+             "wkz_nn_layer_set_training": (some, 1), "wkz_nn_layer_set_step": (some, None),
+             "wkz_nn_token_logprobs_init": (some, some, 8, 2, 4, 0, ctypes.byref(out)), "wkz_nn_token_logprobs_deinit": (some, some),
+             "wkz_nn_token_logprobs_tensor": (some, 0, ctypes.byref(out)), "wkz_nn_token_logprobs_forward": (some, some, some, None),
+             "wkz_nn_token_logprobs_backward": (some, some, some, None, None, None, some), "wkz_nn_loss_tokens": (1, some, some, some, some, some, None)}
+    for name, args in calls.items():
+        missing = [i for i, a in enumerate(args) if a is some]
+        assert missing
+        for i in missing:
+            assert getattr(lib, name)(*(None if k == i else a for k, a in enumerate(args))) == 1, (name, i)
+        with pytest.raises(wekua_amd.WekuaError):
+            wekua_amd._check(getattr(lib, name)(*(None if a is some else a for a in args)), name)

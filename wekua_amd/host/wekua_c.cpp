@@ -73,6 +73,11 @@ template <typename F> int guard(F &&f) {
     }
 }
 
+// handles that a call cannot do without (a layer that was appended to another, a matrix after its deinit have none)
+template <typename... H> void need(const H *...handles) {
+    if ((!handles || ...)) throw Error(WK_E_INVALID_VALUE);
+}
+
 template <typename F> void dispatch(int dtype, F &&f) {
     using namespace wekua::core;
     switch (dtype) {
@@ -736,6 +741,7 @@ int wkz_nn_optimizer_deinit(void *optimizer, void *pipeline) {
 // ---- the token end of a network -----------------------------------------------------------------------------
 int wkz_random_dropout(void *pipeline, void *x, void *y, double p, uint64_t seed, uint64_t offset, void *step) {
     return guard([&] {
+        need(pipeline, x, y);
         TensorHandle *hx = static_cast<TensorHandle *>(x), *hy = static_cast<TensorHandle *>(y), *hs = static_cast<TensorHandle *>(step);
         if (hx->dtype != hy->dtype || (hs && hs->dtype != WK_U64)) throw Error(WK_E_UNQUAL_TENSORS_ATTRIBUTE);
         dispatch_float(hx->dtype, [&]<typename T>() {
@@ -747,15 +753,20 @@ int wkz_random_dropout(void *pipeline, void *x, void *y, double p, uint64_t seed
 
 int wkz_block_scaled_init(void *ctx, void *pipeline, uint64_t rows, uint64_t cols, uint64_t block_rows, void **out) {
     return guard([&] {
+        need(ctx, pipeline);
         if (!out) throw Error(WK_E_INVALID_VALUE);
         *out = blas::BlockScaled::init(static_cast<Context *>(ctx), static_cast<Pipeline *>(pipeline), rows, cols, block_rows);
     });
 }
 int wkz_block_scaled_deinit(void *matrix, void *pipeline) {
-    return guard([&] { static_cast<blas::BlockScaled *>(matrix)->deinit(static_cast<Pipeline *>(pipeline)); });
+    return guard([&] {
+        need(matrix, pipeline);
+        static_cast<blas::BlockScaled *>(matrix)->deinit(static_cast<Pipeline *>(pipeline));
+    });
 }
 int wkz_block_scaled_quantize(void *matrix, void *pipeline, void *x) {
     return guard([&] {
+        need(matrix, pipeline, x);
         TensorHandle *h = static_cast<TensorHandle *>(x);
         dispatch_f8_side(h->dtype, [&]<typename T>() {
             static_cast<blas::BlockScaled *>(matrix)->quantize<T>(static_cast<Pipeline *>(pipeline), static_cast<Tensor<T> *>(h->tensor));
@@ -765,6 +776,7 @@ int wkz_block_scaled_quantize(void *matrix, void *pipeline, void *x) {
 // which: 0 codes, 1 scales; a borrowed handle, for wkz_tensor_handle_drop
 int wkz_block_scaled_tensor(void *matrix, int which, void **out) {
     return guard([&] {
+        need(matrix);
         auto *b = static_cast<blas::BlockScaled *>(matrix);
         if (!out || which < 0 || which > 1) throw Error(WK_E_INVALID_VALUE);
         if (which == 0) *out = new TensorHandle{WK_F8E4M3, b->codes};
@@ -773,6 +785,7 @@ int wkz_block_scaled_tensor(void *matrix, int which, void **out) {
 }
 int wkz_gemm_f8(void *pipeline, void *a, void *b, void *bias, int kind, void *c) {
     return guard([&] {
+        need(pipeline, a, b, c);
         TensorHandle *hb = static_cast<TensorHandle *>(bias), *hc = static_cast<TensorHandle *>(c);
         if (hb && hb->dtype != WK_F32) throw Error(WK_E_UNQUAL_TENSORS_ATTRIBUTE);
         dispatch_f8_side(hc->dtype, [&]<typename O>() {
@@ -784,6 +797,7 @@ int wkz_gemm_f8(void *pipeline, void *a, void *b, void *bias, int kind, void *c)
 
 int wkz_nn_dropout_init(void *ctx, int dtype, uint64_t width, double p, const uint64_t *seed, void **out) {
     return guard([&] {
+        need(ctx);
         if (!out) throw Error(WK_E_INVALID_VALUE);
         dispatch_real(dtype, [&]<typename T>() {
             nn::Layer<T> *l = nn::Dropout<T>::init(static_cast<Context *>(ctx), width, p, seed ? std::optional<uint64_t>(*seed) : std::nullopt);
@@ -793,6 +807,7 @@ int wkz_nn_dropout_init(void *ctx, int dtype, uint64_t width, double p, const ui
 }
 int wkz_nn_layer_set_training(void *layer, int on) {
     return guard([&] {
+        need(layer);
         LayerHandle *h = static_cast<LayerHandle *>(layer);
         dispatch_real(h->dtype, [&]<typename T>() { static_cast<nn::Layer<T> *>(h->layer)->setTraining(on != 0); });
     });
@@ -800,6 +815,7 @@ int wkz_nn_layer_set_training(void *layer, int on) {
 // step: a one-element u64 tensor that stays the caller's, or NULL
 int wkz_nn_layer_set_step(void *layer, void *step) {
     return guard([&] {
+        need(layer);
         LayerHandle *h = static_cast<LayerHandle *>(layer);
         TensorHandle *hs = static_cast<TensorHandle *>(step);
         if (hs && hs->dtype != WK_U64) throw Error(WK_E_UNQUAL_TENSORS_ATTRIBUTE);
@@ -815,6 +831,7 @@ struct TokenLogProbsHandle {
 };
 int wkz_nn_token_logprobs_init(void *ctx, void *pipeline, int dtype, uint64_t rows, uint64_t vocab, uint32_t top, void **out) {
     return guard([&] {
+        need(ctx, pipeline);
         if (!out) throw Error(WK_E_INVALID_VALUE);
         dispatch_float(dtype, [&]<typename T>() {
             *out = new TokenLogProbsHandle{
@@ -824,6 +841,7 @@ int wkz_nn_token_logprobs_init(void *ctx, void *pipeline, int dtype, uint64_t ro
 }
 int wkz_nn_token_logprobs_deinit(void *state, void *pipeline) {
     return guard([&] {
+        need(state, pipeline);
         auto *h = static_cast<TokenLogProbsHandle *>(state);
         dispatch_float(h->dtype, [&]<typename T>() { static_cast<nn::TokenLogProbs<T> *>(h->state)->deinit(static_cast<Pipeline *>(pipeline)); });
         delete h;
@@ -832,6 +850,7 @@ int wkz_nn_token_logprobs_deinit(void *state, void *pipeline) {
 // which: 0 logprob, 1 lse, 2 entropy, 3 top_ids, 4 top_logprobs; NULL where there is none; for wkz_tensor_handle_drop
 int wkz_nn_token_logprobs_tensor(void *state, int which, void **out) {
     return guard([&] {
+        need(state);
         auto *h = static_cast<TokenLogProbsHandle *>(state);
         if (!out || which < 0 || which > 4) throw Error(WK_E_INVALID_VALUE);
         dispatch_float(h->dtype, [&]<typename T>() {
@@ -844,6 +863,7 @@ int wkz_nn_token_logprobs_tensor(void *state, int which, void **out) {
 }
 int wkz_nn_token_logprobs_forward(void *state, void *pipeline, void *logits, void *targets) {
     return guard([&] {
+        need(state, pipeline, logits);
         auto *h = static_cast<TokenLogProbsHandle *>(state);
         TensorHandle *hl = static_cast<TensorHandle *>(logits), *ht = static_cast<TensorHandle *>(targets);
         if (hl->dtype != h->dtype) throw Error(WK_E_UNQUAL_TENSORS_ATTRIBUTE);
@@ -860,6 +880,7 @@ int wkz_nn_token_logprobs_forward(void *state, void *pipeline, void *logits, voi
 int wkz_nn_token_logprobs_backward(void *state, void *pipeline, void *logits, void *targets, void *logprob_grad, void *entropy_grad,
                                    void *logits_grad) {
     return guard([&] {
+        need(state, pipeline, logits, logits_grad);
         auto *h = static_cast<TokenLogProbsHandle *>(state);
         TensorHandle *hl = static_cast<TensorHandle *>(logits), *ht = static_cast<TensorHandle *>(targets),
                      *hw = static_cast<TensorHandle *>(logprob_grad), *he = static_cast<TensorHandle *>(entropy_grad),
@@ -883,6 +904,7 @@ int wkz_nn_token_logprobs_backward(void *state, void *pipeline, void *logits, vo
 int wkz_nn_loss_tokens(int calculate_derivative, void *pipeline, void *output, void *targets, void *state, void *cache,
                        void *host_error_result) {
     return guard([&] {
+        need(pipeline, output, targets, state, cache);
         CacheHandle *hc = static_cast<CacheHandle *>(cache);
         auto *hs = static_cast<TokenLogProbsHandle *>(state);
         TensorHandle *ho = static_cast<TensorHandle *>(output), *ht = static_cast<TensorHandle *>(targets);
