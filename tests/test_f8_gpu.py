@@ -110,6 +110,40 @@ def test_gemm_sizes(dev, M, N, K):
     check_gemm(dev, M, N, K, pads=(1 if K % 16 == 0 else 0, 0, 0))
 
 
+@pytest.mark.parametrize("out", ["f16", "bf16"])
+@pytest.mark.parametrize("M,N,K", [(65, 70, 1), (100, 100, 100), (65, 300, 129), (129, 127, 384), (257, 511, 640), (300, 200, 2049), (150, 150, 9001), (1000, 140, 255)])
+def test_gemm_any_address_16_bit(dev, out, M, N, K):
+    """16-bit results of more than 64 rows whose operands' rows begin anywhere: the register-staged tiles with the 8-bit instruction."""
+    check_gemm(dev, M, N, K, out, pads=(1 if K % 16 == 0 else 0, 0, 0))
+    check_gemm(dev, M, N, K, out, True, 1, pads=(3, 2, 1), shift=7)
+
+
+@pytest.mark.parametrize("M,N,K,kind", [(2048, 192, 1100, 1), (3600, 3700, 136, -1), (3840, 3584, 640, -1), (3601, 3900, 1280, 0), (700, 2100, 520, -1)])
+def test_gemm_large_f16(dev, M, N, K, kind):
+    check_gemm(dev, M, N, K, "f16", kind == 0, kind, pads=(-K % 16, -K % 16, 4 if M % 2 else 0), cut=False)
+
+
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("M,N,K", [(8, 2048, 4096), (1000, 1300, 2000), (4096, 4096, 4096)])
+def test_gemm_same_bits_on_every_run(dev, out, M, N, K):
+    """Ten runs one after the other, into buffers that hold something else each time."""
+    rng = np.random.RandomState(M)
+    kb, ld = -(-K // 128), -(-K // 16) * 16
+    a, b = (rng.randint(0, 0x7F, (r, ld)).astype(np.uint8) | (rng.randint(0, 2, (r, ld)) << 7).astype(np.uint8) for r in (M, N))
+    bufs = [dev.upload(v) for v in (a, b, np.exp(rng.randn(M, kb)).astype(np.float32), np.exp(rng.randn(-(-N // 128), kb)).astype(np.float32))]
+    t = np.uint32 if out == "f32" else np.uint16
+    first = None
+    for run in range(10):
+        bc = dev.upload(np.full((M, N), run, t))
+        dev.gemm_f8(M, N, K, bufs[0], ld, bufs[2], kb, bufs[1], ld, bufs[3], kb, out, bc, N)
+        got = bc.download(t, (M, N))
+        assert first is None or np.array_equal(got, first), run
+        first = got
+        bc.free()
+    for x in bufs:
+        x.free()
+
+
 @pytest.mark.parametrize("out", ["f32", "bf16"])
 @pytest.mark.parametrize("M,N,K,kind", [(65, 16, 128, -1), (2048, 192, 1100, 1), (3600, 3700, 136, -1), (3840, 3584, 640, -1), (3601, 3900, 1280, 0), (1, 20000, 512, -1)])
 def test_gemm_large(dev, out, M, N, K, kind):
@@ -130,6 +164,14 @@ def test_gemm_few_rows_many_columns(dev, out, M, N, K):
 @pytest.mark.parametrize("M,N", [(3, 70), (200, 300)])
 def test_gemm_epilogue(dev, out, bias, kind, M, N):
     check_gemm(dev, M, N, 272, out, bias, kind, pads=(0, 0, 1))
+
+
+@pytest.mark.parametrize("out", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shift", [1, 2, 4, 8, 15])
+def test_gemm_unaligned_bases_in_tiles(dev, out, shift):
+    """More than 64 rows behind a base that is no multiple of 16, rows a multiple of 16 apart and not."""
+    check_gemm(dev, 130, 150, 256, out, shift=shift)
+    check_gemm(dev, 70, 200, 300, out, shift=shift, pads=(4, 20, 0))
 
 
 @pytest.mark.parametrize("out", ["f32", "bf16"])

@@ -518,6 +518,20 @@ def same(a, b):
     return all(np.array_equal(a[n], b[n], equal_nan=True) for n in a)
 
 
+def test_products_of_the_run(dev):
+    """Both products of the run against 64 bits: what the tests below compare runs with."""
+    step = Step(dev, 7)
+    step()
+    got, k = step.results(), step.blocks
+    wq, ws = ot.f8_quantize(step.w.astype(np.float64), 128)
+    rq, rs = ot.f8_quantize(step.w.astype(np.float64), 1)
+    for name, a, sa, out in (("c", got["gq"], got["gs"], "f32"), ("big", rq, rs, "bf16")):
+        want, mag, largest = ot.gemm_f8(a, sa, wq, ws)
+        tol = (128 + k + 2) * 2.0 ** -23 * mag + (7 * 2.0 ** -13 * largest + 2.0 ** -8 * 1.01 * np.abs(want) if out != "f32" else 2.0 ** -24 * np.abs(want))
+        assert (np.abs(values(out, got[name]) - want) <= tol + 1e-37).all(), name
+    step.free()
+
+
 def test_run_on_two_streams_at_once(dev):
     """Two runs at once, on two streams, give what each gives alone; and so does the same one twice."""
     from wekua_amd import raw
