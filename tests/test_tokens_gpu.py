@@ -164,6 +164,47 @@ def test_ties_across_the_whole_row(dev):
             assert np.array_equal(got["top_ids"], ot.token_logprobs(values(dtype, bits), None, 64)["top_ids"])
 
 
+@pytest.mark.parametrize("dtype,rows,vocab,top", [("bf16", 2100, 33001, 5), ("f32", 1050, 33003, 64), ("f32", 600, 60001, 20), ("f64", 40, 430001, 7)])
+def test_logits_that_pass_the_cache_by(dev, dtype, rows, vocab, top):
+    """More than 128 MB of logits with alternatives, rows whole and cut: thirty rows in turn, of which the copies have the same bits."""
+    rng = np.random.RandomState(rows)
+    block = pack(dtype, logits(rng, 30, vocab))
+    if dtype != "bf16":
+        block[3, rng.rand(vocab) < 0.9] = -np.inf
+    t = rng.randint(0, vocab, 30)
+    bits, targets = np.resize(block, (rows, vocab)), np.resize(t, rows)
+    assert bits.nbytes > 128 << 20
+    got = run_forward(dev, dtype, bits, targets, top, 1)
+    check_forward({n: v[:30] for n, v in got.items()}, dtype, values(dtype, block), t, top)
+    for v in got.values():
+        assert np.array_equal(v, np.resize(v[:30], v.shape), equal_nan=True)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f64", "bf16"])
+@pytest.mark.parametrize("rows,vocab,top", [(1, 131072, 20), (3, 20011, 0), (2, 9001, 64)])
+def test_a_workspace_that_is_too_small(dev, dtype, rows, vocab, top):
+    """Less than the call asks for is as good as none: the same bits, and nothing is written there."""
+    rng = np.random.RandomState(rows)
+    acc = np.float64 if dtype == "f64" else np.float32
+    bits, t = pack(dtype, logits(rng, rows, vocab)), rng.randint(0, vocab, rows).astype(np.int32)
+    n = dev.token_logprobs_workspace_bytes(dtype, rows, vocab, top)
+    assert n
+    bx, bt, ws = dev.upload(bits), dev.upload(t), dev.upload(np.full(n, 0xFF, np.uint8))
+    stats, ids, lps = [dev.malloc(rows * acc().itemsize) for _ in range(3)], dev.malloc(4 * rows * top + 4), dev.malloc(8 * rows * top + 8)
+    seen = []
+    for space, size in ((None, 0), (ws, 0), (ws, 16), (ws, n - 1)):
+        dev.token_logprobs(dtype, rows, vocab, bx, vocab, bt, "i32", *stats, top, ids if top else None, lps if top else None, space, size)
+        seen.append([b.download(acc, (rows,)) for b in stats] + ([ids.download(np.int32, (rows, top)), lps.download(acc, (rows, top))] if top else []))
+    for other in seen[1:]:
+        assert all(np.array_equal(a, b) for a, b in zip(seen[0], other))
+    assert (ws.download(np.uint8, (n,)) == 0xFF).all()
+    got = dict(zip(("logprob", "lse", "entropy"), seen[0][:3]), top_ids=seen[0][3] if top else np.zeros((rows, 0), np.int32),
+               top_logprobs=seen[0][4] if top else np.zeros((rows, 0), acc))
+    check_forward(got, dtype, values(dtype, bits), t, top)
+    for b in (bx, bt, ws, ids, lps, *stats):
+        b.free()
+
+
 @pytest.mark.parametrize("outputs", [("logprob",), ("lse",), ("entropy",), ("logprob", "entropy"), ()])
 def test_only_what_is_wanted(dev, outputs):
     rng = np.random.RandomState(8)
