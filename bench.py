@@ -5,7 +5,9 @@ A "step" is one call of the headline workload: f32 GEMM C = 1.5*A*B + 0.5*C at
 M = N = K = 8192 (no transposes), operands resident in HBM.  The AXPY half of the metric
 (y = 0.75*x + y, f32, n = 2^28) is measured in the same run and reported beside it.
 
-Prints ONE JSON line:
+Prints ONE JSON line (figures to six digits, of the other workloads the rates alone, so that it stays below LINE_LIMIT characters and
+whoever keeps the end of the output keeps all of it; --record FILE writes everything, CPU baselines, batches and bounds of every workload
+among it):
   metric / value / unit   as the benchmark definition names them (the headline GEMM, wall clock);
   roofline                the headline GEMM kernel against the f32 matrix peak, from events on its stream;
   axpy                    f32 / f64 at n = 2^28 against the HBM peak, the same kernel under two placements
@@ -41,8 +43,34 @@ FLOOR_GEMM_TFLOPS = 130.0        # f32 8192^3 NN (measured 139-144 across boxes)
 FLOOR_AXPY_GBS = 6600.0          # f32 n = 2^28 (measured 6820-6860 across boxes)
 
 
+LINE_LIMIT = 10000
+
+
 def log(*a):
     print(*a, file=sys.stderr, flush=True)
+
+
+def short(v, digits=6):
+    """Every float of a record to `digits` significant digits."""
+    if isinstance(v, dict):
+        return {k: short(x, digits) for k, x in v.items()}
+    if isinstance(v, (list, tuple)):
+        return [short(x, digits) for x in v]
+    return v if not isinstance(v, float) else int(v) if v.is_integer() else float(f"{v:.{digits}g}")
+
+
+def one_line(record):
+    """The line that is printed of a whole record: of the lists of workloads what was reached and by which kernel, in four digits."""
+    out = dict(record)
+    for key in ("configs", "off_benchmark_sizes"):
+        if record.get(key):
+            out[key] = {name: short({k: r.get(k) for k in ("value", "unit", "kernel") if r.get(k) is not None}
+                                    | ({"frac": r["roofline"]["frac"]} if isinstance(r.get("roofline"), dict) else {}), 4)
+                        for name, r in record[key].items()}
+    out["cpu_baselines"] = {name: short({k: r[k] for k in ("value", "unit")}, 4) for name, r in (record.get("cpu_baselines") or {}).items()} or None
+    out["axpy"] = {k: {n: x for n, x in v.items() if n not in ("what", "sample")} if isinstance(v, dict) else v for k, v in record["axpy"].items()
+                   if k not in ("over_batches", "f64_over_batches")}
+    return json.dumps(short(out), separators=(",", ":"))
 
 
 def read_traffic(name: str, kernel: str):
@@ -236,6 +264,7 @@ def main():
     ap.add_argument("--no-mlp", action="store_true", help="skip the MLP training step leg (benchmark configuration 5)")
     ap.add_argument("--no-configs", action="store_true", help="skip the sweep over the other benchmark configurations")
     ap.add_argument("--no-floor", action="store_true", help="do not turn a missed performance floor into exit status 3")
+    ap.add_argument("--record", default=None, help="write everything that was measured to this file, as JSON")
     args = ap.parse_args()
     if args.gpus != 1:
         print("bench.py: this build uses one GPU; --gpus N with N > 1 is not supported "
@@ -371,7 +400,10 @@ def main():
         "cpu_baselines": cpu_all,
         "perf_floor": floor,
     }
-    print(json.dumps(out), flush=True)
+    if args.record:
+        with open(args.record, "w") as f:
+            json.dump(out, f, indent=1)
+    print(one_line(out), flush=True)
     if not floor_ok and not args.no_floor:
         log(f"[bench] below the performance floor: {floor}")
         sys.exit(3)
