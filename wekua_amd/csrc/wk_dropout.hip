@@ -49,7 +49,9 @@ typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2))); // 1
 // One thread takes PER consecutive elements of a row, 16 bytes (f64: 32), loaded before their words are drawn.  PHASE0: every row
 // begins at a multiple of four elements, so the PER words are whole blocks; otherwise a row's first word is
 // (row * cols) % 4 words into its block and one block more is drawn.  STREAM: the tensors fill the last-level cache (256 MB)
-// or more and pass it by.
+// or more and pass it by.  (Two pairs of tensors in turn, so that nothing is found there, f32, us without and with it: 128 MB a pair 20.6 and
+// 22.2, 160 MB 30.1 and 28.2, 224 MB 41.0 and 37.8, 256 MB 45.3 and 42.4, 320 MB 57.3 and 52.8.  Below 256 MB a pair fits, and
+// what comes next may find it there.)
 // Bound by memory, with the words' multiplications close behind: 8192 x 8192 bf16 43 us each way (6.2 TB/s), 45 with
 // plain loads and stores, 65 where the words were drawn first; 16 x 1024 f32 2.5 us, a launch.
 template <typename T, int PER, bool PHASE0, bool STREAM>

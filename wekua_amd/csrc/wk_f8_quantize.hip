@@ -72,7 +72,9 @@ __device__ __forceinline__ void store8(uint8_t *p, uint64_t left, const float v[
 
 // STREAM, here and below: the last-level cache (256 MB) would not hold x and what comes next, so x passes it by, and what lies there
 // unwritten need not be put out for it.  Measured (8192 x 8192, us) with a cache full of other writes, then without: per block
-// f32 90 -> 65 and 62 -> 61, bf16 64 -> 42 and 37 -> 37; 4096 x 4096 f32, which it holds, 15 -> 19.  The codes stay in
+// f32 90 -> 65 and 62 -> 61, bf16 64 -> 42 and 37 -> 37; 4096 x 4096 f32, which it holds, 15 -> 19.  With two matrices in turn, 128 x 128
+// blocks: f32 96 MB 20.2 -> 24.5, 128 MB 30.7 -> 31.6, 160 MB 39.0 -> 38.3, 256 MB 60.7 -> 57.9; bf16 64 MB 17.4 -> 18.9, 96 MB 29.0 -> 25.9,
+// 128 MB 37.3 -> 32.8, 160 MB 45.8 -> 40.2 (bf16 would want the border nearer 80 MB; it is the f32 one).  The codes stay in
 // the cache for the product: past it, another 5 us less here were 13 more there.
 //
 // One scale per row and 128 columns: sixteen lanes to a block, sixteen blocks to a work-group.  Bound by memory: 8192 x 8192 f32

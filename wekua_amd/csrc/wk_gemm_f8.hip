@@ -224,10 +224,13 @@ template <typename O> __global__ __launch_bounds__(256, 2) void gemm_f8_tile_ker
 //
 // 16-bit results, 8192^3: 510 us, 2.15 PFLOP/s (a library product of tensors with one scale 398); matrix instructions run half
 // of the time at a clock that the power limit holds near 1.9 GHz.  A block takes 4000 cycles: 2048 of products, and as many of the LDS port
-// (192 KB of operands to eight wavefronts, 64 KB that arrive; without the arrivals 428 us, without the barrier 500).  f32: 1090 us, 1.0 PFLOP/s (the library's f16 product 770).  There the vector
-// instructions are the bound: of 2400 cycles to a block of a 128 x 128 tile 1024 are products, and with them 128 widenings of
-// two codes at 8 cycles, 64 multiply-adds and what moves data have to be issued; taking turns with the products brought 2580 to
-// that.  Tiles of 128 x 256 widen a quarter less, but their sums do not fit the 256 registers that vector instructions reach.
+// (192 KB of operands to eight wavefronts, 64 KB that arrive; without the arrivals 428 us, without the barrier 500).
+//
+// f32, 8192^3: 1090 us, 1.0 PFLOP/s (the library's f16 product 770).  Neither pipe is full: counted when a block of a 128 x 128
+// tile alone on its unit took 2580 cycles (2400 since the loads need no wait states), 1024 were products and 1124 issued vector instructions
+// (128 widenings of two codes at 8 cycles, 64 multiply-adds and what moves data); 530 a wavefront waited, 608 it waited for its turn
+// to issue.  Two such work-groups on a unit do not overlap the two either (148 us for both, 79 for one).
+// Tiles of 128 x 256 widen a quarter less, but their sums do not fit the 256 registers that vector instructions reach.
 template <typename O, int WM, int WN, int MT, int NT, int STAGES> struct DmaTile {
     static constexpr uint32_t TM = WM * MT * 16, TN = WN * NT * 16, THREADS = WM * WN * 64;
     static constexpr uint32_t NB = TN > KB ? TN / KB : 1; // rows of B's scales

@@ -66,9 +66,9 @@ inline int hip_code(hipError_t e) {
         }                                                 \
     } while (0)
 
-// Every launch is followed by this: a bad launch configuration surfaces here, not later.
-// the work-groups that one launch may have: its threads are counted in 32 bits
+// The work-groups that one launch may have: its threads are counted in 32 bits.
 constexpr uint64_t most_groups(uint32_t threads) { return 0xffffffffull / threads; }
+// Every launch is followed by this: a bad launch configuration surfaces here, not later.
 inline int launch_status() { return hip_code(hipGetLastError()); }
 
 // Looks up this device's address of the static scratch array of wk_bias_step_static (wk_nn.hip);

@@ -476,6 +476,8 @@ void logprobs_enqueue(hipStream_t st, unsigned grid, const T *x, uint64_t pitch,
                       uint32_t parts, uint32_t top, const Outputs<typename stat_of<T>::type> &o, typename stat_of<T>::type *ws, int32_t *ids) {
     // Logits of which the last-level cache (256 MB) would not keep enough until the backward pass go by it: 8192 x 32000 f32
     // 177 -> 154 us, 2048 x 50021 bf16 with alternatives 52 -> 48; below half of the cache what was just written is found there.
+    // Two sets of logits in turn, without and with it: f32 96 MB 19.0 and 18.4, 128 MB 23.8 and 23.8, 160 MB 31.4 and 28.7, 256 MB 48.4
+    // and 43.7; bf16 128 MB 30.5 and 30.7, 160 MB 38.0 and 37.6, 256 MB 58.6 and 56.5.
     const bool stream = rows * vocab * sizeof(T) > (128ull << 20);
     const dim3 block(WAVES == 1 ? 256 : WAVES * 64);
     if (top)
@@ -526,7 +528,8 @@ template <typename A> struct GradArgs {
 
 // One thread takes GRAD_DEEP x 16 bytes of a row, all loads issued before any is used; blockIdx.x counts a row's segments first.
 // STREAM: both tensors together are more than the last-level cache holds (256 MB), so that neither is kept there: 4096 x 65536 bf16
-// 190 -> 171 us (6.3 TB/s), where 1000 x 32003 f32, which it half holds, loses (39 -> 45).  Two loads in flight per thread did
+// 190 -> 167 us (6.4 TB/s), where 1000 x 32003 f32, which it half holds, loses (39 -> 45; two sets of both in turn: 128 MB 21.4 -> 24.6,
+// 160 MB 32.5 -> 29.7, 224 MB 43.4 -> 39.8, 320 MB 59.3 -> 54.8).  Two loads in flight per thread did
 // better than one, four and eight (171 against 175, 180 and 185).
 template <typename T, bool ENTROPY, bool STREAM>
 __global__ __launch_bounds__(256) void logprobs_grad_kernel(const T *x, uint64_t pitch, T *dx, uint64_t grad_pitch, uint32_t vocab,

@@ -499,7 +499,8 @@ template <typename T> struct Cache {
 
 // ---- log probabilities of tokens (no counterpart in the reference) --------------------------------------
 // Results and workspace of wk_token_logprobs for {rows, vocab} logits: for scoring and serving (with the `top` likeliest
-// tokens) and for training.  T: f32, f64, F16, BF16; results are f32 (f64 for f64).
+// tokens) and for training.  T: f32, f64, F16, BF16; results are f32 (f64 for f64).  Both are overwritten by the next forward
+// pass: passes on one object are for one pipeline, or ordered.
 template <typename T> struct TokenLogProbs {
     using S = std::conditional_t<std::is_same_v<T, double>, double, float>;
     uint64_t rows = 0, vocab = 0;

@@ -216,7 +216,8 @@ class Cache:
 
 class TokenLogProbs:
     """Log probabilities of given tokens over {rows, vocab} logits with entropy and the `top` likeliest tokens, and their
-    gradient.  dtype (of the logits): f32, f64, f16, bf16; results are f32 (f64 for f64).  No counterpart in the reference."""
+    gradient.  dtype (of the logits): f32, f64, f16, bf16; results are f32 (f64 for f64).  Results and workspace are overwritten by the
+    next forward pass, so passes on one object are for one pipeline, or ordered.  No counterpart in the reference."""
 
     def __init__(self, handle, dtype: str, context, rows: int, top: int):
         self._h = handle
