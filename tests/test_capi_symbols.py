@@ -335,3 +335,18 @@ def test_missing_handles_are_refused():
             assert getattr(lib, name)(*(None if k == i else a for k, a in enumerate(args))) == 1, (name, i)
         with pytest.raises(wekua_amd.WekuaError):
             wekua_amd._check(getattr(lib, name)(*(None if a is some else a for a in args)), name)
+
+
+def test_values_are_not_taken_for_bits():
+    """A bf16 or f8e4m3 tensor is filled with bits: an array of numbers is refused before anything is copied (cast to the bits' whole
+    numbers it would be other values)."""
+    import types
+    import numpy as np
+    from wekua_amd import memory
+    for dtype, others in (("bf16", (np.float32, np.float16, np.float64, np.int64, np.int16)), ("f8e4m3", (np.float32, np.uint16, np.int8))):
+        tensor = types.SimpleNamespace(dtype=dtype, _h=None)
+        for other in others:
+            with pytest.raises(TypeError):
+                memory.readFromBuffer(types.SimpleNamespace(_h=None), tensor, np.ones(4, other))
+        with pytest.raises(TypeError):
+            memory.readFromBuffer(types.SimpleNamespace(_h=None), tensor, [1.5, 2.5])

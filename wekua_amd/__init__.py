@@ -315,7 +315,10 @@ class Tensor:
 class memory:
     @staticmethod
     def readFromBuffer(pipeline: Pipeline, tensor: Tensor, buffer: np.ndarray) -> None:
-        """HOST -> DEVICE; `buffer` holds exactly the logical elements (complex: trailing (re, im) axis)."""
+        """HOST -> DEVICE; `buffer` holds exactly the logical elements (complex: trailing (re, im) axis), of bf16 and f8e4m3 their bits
+        (uint16, uint8)."""
+        if tensor.dtype in ("bf16", "f8e4m3") and np.asarray(buffer).dtype != real_np_dtype(tensor.dtype):
+            raise TypeError(f"readFromBuffer takes the bits of {tensor.dtype}, an array of {real_np_dtype(tensor.dtype)}")
         buffer = np.ascontiguousarray(buffer, dtype=real_np_dtype(tensor.dtype))
         n = buffer.size // (2 if is_complex(tensor.dtype) else 1)
         _check(_lib().wkz_read_from_buffer(pipeline._h, tensor._h, buffer.ctypes.data, n), "memory.readFromBuffer")
