@@ -350,3 +350,24 @@ def test_values_are_not_taken_for_bits():
                 memory.readFromBuffer(types.SimpleNamespace(_h=None), tensor, np.ones(4, other))
         with pytest.raises(TypeError):
             memory.readFromBuffer(types.SimpleNamespace(_h=None), tensor, [1.5, 2.5])
+
+
+def test_operands_that_are_elsewhere_or_gone():
+    """raw.Device hands no host memory, no other device's and nothing that was freed to a kernel, nor an absent operand in its place."""
+    import types
+    import torch
+    from wekua_amd import raw
+    dev = object.__new__(raw.Device)
+    dev.ordinal = 0
+
+    def buffer(ptr, ordinal=0):
+        b = object.__new__(raw.DeviceBuffer)
+        b.ptr, b.device = ptr, types.SimpleNamespace(ordinal=ordinal)
+        return b
+    here = types.SimpleNamespace(data_ptr=lambda: 4096, get_device=lambda: 0)
+    assert dev._address(None) is None and dev._address(4096) == 4096 and dev._address(here) == 4096
+    assert dev._address(types.SimpleNamespace(data_ptr=lambda: 4096)) == 4096 and dev._address(buffer(ctypes.c_void_p(4096))).value == 4096
+    for bad in (torch.ones(4), torch.empty(0), types.SimpleNamespace(data_ptr=lambda: 4096, get_device=lambda: 1),
+                types.SimpleNamespace(data_ptr=lambda: 0, get_device=lambda: 0), buffer(None), buffer(ctypes.c_void_p(4096), 1)):
+        with pytest.raises(ValueError):
+            dev._address(bad)

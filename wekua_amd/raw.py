@@ -59,18 +59,12 @@ def scalar_bytes(name: str, value):
     return ctypes.create_string_buffer(arr.tobytes(), arr.nbytes)
 
 
-def _address(buf):
-    """The device address of a DeviceBuffer, of anything with data_ptr(), or a plain address; None stays None."""
-    if buf is None or isinstance(buf, int):
-        return buf
-    return buf.data_ptr() if hasattr(buf, "data_ptr") else buf.ptr
-
-
 class Device:
     """One GPU and one in-order stream on it."""
 
     def __init__(self, ordinal: int = 0):
         self.lib = _capi.load()
+        self.ordinal = ordinal
         self.dev = ctypes.c_void_p()
         check(self.lib.wk_device_open(ordinal, ctypes.byref(self.dev)), "wk_device_open")
         self.stream = ctypes.c_void_p()
@@ -146,23 +140,36 @@ class Device:
     # -- the token end of a network ---------------------------------------------------------
     # Buffers: DeviceBuffers, device addresses, or objects with data_ptr() whose memory is on this device and ready on
     # this stream (work of another stream on them is the caller's to wait for).
+    def _address(self, buf):
+        """The device address of a DeviceBuffer, of anything with data_ptr(), or a plain address; None (an operand that is not there) stays
+        None.  Memory that is known to be elsewhere, or gone, is refused: the kernel would fault, or take it for an absent operand."""
+        if buf is None or isinstance(buf, int):
+            return buf
+        if hasattr(buf, "data_ptr"):
+            at, where = buf.data_ptr(), buf.get_device() if hasattr(buf, "get_device") else self.ordinal
+        else:
+            at, where = buf.ptr, buf.device.ordinal
+        if not at or where != self.ordinal:
+            raise ValueError("an operand has no memory" if not at else f"an operand is not on device {self.ordinal}")
+        return at
+
     def dropout(self, dtype: str, shape3, x, xrp: int, xsp: int, y, yrp: int, ysp: int, p: float, seed: int, offset: int = 0,
                 step=None) -> None:
         """wk_dropout; the backward pass is the same call on the gradient."""
-        check(self.lib.wk_dropout(self.stream, dtype_id(dtype), (ctypes.c_uint64 * 3)(*shape3), _address(x), xrp, xsp, _address(y), yrp, ysp,
-                                  p, seed, offset, _address(step)), "wk_dropout")
+        check(self.lib.wk_dropout(self.stream, dtype_id(dtype), (ctypes.c_uint64 * 3)(*shape3), self._address(x), xrp, xsp,
+                                  self._address(y), yrp, ysp, p, seed, offset, self._address(step)), "wk_dropout")
 
     def f8_quantize(self, dtype: str, rows: int, cols: int, x, pitch: int, block_rows: int, q, q_pitch: int, scales,
                     scale_pitch: int) -> None:
         """wk_f8_quantize: 8-bit codes and a scale for each block of block_rows (1 or 128) x 128 elements."""
-        check(self.lib.wk_f8_quantize(self.stream, dtype_id(dtype), rows, cols, _address(x), pitch, block_rows, _address(q), q_pitch,
-                                      _address(scales), scale_pitch), "wk_f8_quantize")
+        check(self.lib.wk_f8_quantize(self.stream, dtype_id(dtype), rows, cols, self._address(x), pitch, block_rows, self._address(q), q_pitch,
+                                      self._address(scales), scale_pitch), "wk_f8_quantize")
 
     def gemm_f8(self, M: int, N: int, K: int, A, lda: int, a_scales, a_scale_pitch: int, B, ldb: int, b_scales, b_scale_pitch: int,
                 out_dtype: str, C, ldc: int, bias=None, kind: int = -1) -> None:
         """wk_gemm_f8: C = act(A B^T + bias) of 8-bit operands with block scales."""
-        check(self.lib.wk_gemm_f8(self.stream, M, N, K, _address(A), lda, _address(a_scales), a_scale_pitch, _address(B), ldb,
-                                  _address(b_scales), b_scale_pitch, dtype_id(out_dtype), _address(C), ldc, _address(bias), kind), "wk_gemm_f8")
+        check(self.lib.wk_gemm_f8(self.stream, M, N, K, self._address(A), lda, self._address(a_scales), a_scale_pitch, self._address(B), ldb,
+                                  self._address(b_scales), b_scale_pitch, dtype_id(out_dtype), self._address(C), ldc, self._address(bias), kind), "wk_gemm_f8")
 
     def token_logprobs_workspace_bytes(self, dtype: str, rows: int, vocab: int, top: int = 0) -> int:
         return int(self.lib.wk_token_logprobs_workspace_bytes(dtype_id(dtype), rows, vocab, top))
@@ -171,16 +178,16 @@ class Device:
                        lse=None, entropy=None, top: int = 0, top_ids=None, top_logprobs=None, workspace=None,
                        workspace_bytes: int = 0) -> None:
         """wk_token_logprobs; outputs that are None are not computed."""
-        check(self.lib.wk_token_logprobs(self.stream, dtype_id(dtype), rows, vocab, _address(logits), pitch, _address(targets),
-                                         dtype_id(target_dtype), _address(logprob), _address(lse), _address(entropy), top,
-                                         _address(top_ids), _address(top_logprobs), _address(workspace), workspace_bytes), "wk_token_logprobs")
+        check(self.lib.wk_token_logprobs(self.stream, dtype_id(dtype), rows, vocab, self._address(logits), pitch, self._address(targets),
+                                         dtype_id(target_dtype), self._address(logprob), self._address(lse), self._address(entropy), top,
+                                         self._address(top_ids), self._address(top_logprobs), self._address(workspace), workspace_bytes), "wk_token_logprobs")
 
     def token_logprobs_grad(self, dtype: str, rows: int, vocab: int, logits, pitch: int, targets, target_dtype: str, lse, entropy,
                             logprob_grad, entropy_grad, logits_grad, grad_pitch: int) -> None:
         """wk_token_logprobs_grad: the gradient of the logits from those of the log probabilities and entropies."""
-        check(self.lib.wk_token_logprobs_grad(self.stream, dtype_id(dtype), rows, vocab, _address(logits), pitch, _address(targets),
-                                              dtype_id(target_dtype), _address(lse), _address(entropy), _address(logprob_grad),
-                                              _address(entropy_grad), _address(logits_grad), grad_pitch), "wk_token_logprobs_grad")
+        check(self.lib.wk_token_logprobs_grad(self.stream, dtype_id(dtype), rows, vocab, self._address(logits), pitch, self._address(targets),
+                                              dtype_id(target_dtype), self._address(lse), self._address(entropy), self._address(logprob_grad),
+                                              self._address(entropy_grad), self._address(logits_grad), grad_pitch), "wk_token_logprobs_grad")
 
 
 class DeviceBuffer:
