@@ -338,8 +338,8 @@ int  wk_f8_quantize(wk_stream *s, int dtype, uint64_t rows, uint64_t cols, const
  * Bases and leading dimensions may be any.  On 16-byte boundaries (multiples of 16) the faster kernels take products of more than
  * 64 rows, of 16384 columns and more, and for 16-bit results of more than 16 rows; the others are fastest on 4-byte ones.
  * On 16-byte boundaries operands are read in whole 16 bytes: up to the next multiple of 16 behind the K-th code of a row, the last
- * one too, which so has to be readable memory; what it holds has no effect.  Otherwise nothing behind a row is read.  B turned around (for the gradient of the input) is wk_transpose of its codes and, for
- * 128 x 128 blocks, of its scales. */
+ * one too, which so has to be readable memory; what it holds has no effect.  Otherwise nothing behind a row is read.
+ * B turned around (for the gradient of the input) is wk_transpose of its codes and, for 128 x 128 blocks, of its scales. */
 int  wk_gemm_f8(wk_stream *s, uint64_t M, uint64_t N, uint64_t K, const void *A, uint64_t lda, const float *a_scales,
                 uint64_t a_scale_pitch, const void *B, uint64_t ldb, const float *b_scales, uint64_t b_scale_pitch, int out_dtype,
                 void *C, uint64_t ldc, const float *bias, int kind);
